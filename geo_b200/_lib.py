@@ -87,6 +87,16 @@ def lib():
     L.geo_sc_guide_backward_bytes.argtypes = [dp, szp]
     L.geo_sc_guide_backward.argtypes = [dp, vp, vp, vp, vp, vp, vp, sz, vp]
     L.geo_sc_guide_backward_quantized.argtypes = [dp, vp, vp, vp, vp, vp, vp, sz, vp]
+    i64 = ctypes.c_longlong
+    L.geo_sc_rms_norm_int8.argtypes = [i64, i32, i32, vp, i64, vp, i64, vp, i32, f32, vp, vp, i64, vp, vp]
+    L.geo_sc_quantize_int8.argtypes = [i64, i32, i32, vp, i64, vp, i64, vp, vp]
+    L.geo_sc_dequantize_int8.argtypes = [i64, i32, vp, i64, vp, i32, vp, vp]
+    L.geo_sc_linear_int8.argtypes = [i32, i32, i32, vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, vp]
+    L.geo_sc_distill_forward.argtypes = [i64, i32, i32, i32, vp, i64, vp, i32, vp, i32, vp, f32, f32, i32, vp, vp, vp, vp, vp]
+    L.geo_sc_distill_backward.argtypes = [i64, i32, i32, i32, vp, i64, vp, i32, vp, i32, vp, f32, f32, i32, vp, vp, i32, vp, vp]
+    for n in ("geo_sc_rms_norm_int8", "geo_sc_quantize_int8", "geo_sc_dequantize_int8", "geo_sc_linear_int8",
+              "geo_sc_distill_forward", "geo_sc_distill_backward"):
+        getattr(L, n).restype = i32
     L.geo_sc_measure_lop3_peak.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
     for n in ("geo_sc_conv2d_forward", "geo_sc_linear_forward", "geo_sc_prepare_weights",
               "geo_sc_generate_act_streams", "geo_sc_accumulate", "geo_sc_group_geometry", "geo_sc_host_stream",

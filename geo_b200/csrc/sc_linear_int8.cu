@@ -1,0 +1,121 @@
+// 8-bit matrix product with a scale per token and per output channel:
+//
+//   out[m][n] = (sum_k x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]
+//
+// The sum is exact in 32-bit integers (k <= 131071, so that 2^14 k stays below 2^31); the two scales and the bias are
+// applied in fp32 and the result is rounded once to the output's type.
+//
+// linear_int8_mma_kernel: `mma.sync.m16n8k32` with the weights as the 16-row operand, read once from memory straight
+// into fragments.  The order of k inside a product is free, so a lane takes 16 consecutive bytes of its weight row and
+// the same 16 bytes of its token rows for two instructions: whole 16-byte loads, no shared memory, no shuffles.  A CTA
+// of eight warps owns 16 channels x 8 * NT tokens; the warps split k and join their integer sums in shared memory.
+#include "sc_rows8.h"
+
+namespace geo {
+namespace {
+
+struct LinearParams {
+    const int8_t *x, *w;
+    const float *x_scale, *w_scale, *bias;
+    void *out;
+    long long x_stride, w_stride, out_stride;
+    int m, n, k;
+};
+
+// 16 bytes of a row from byte `at` on, zeros from byte k on.
+__device__ __forceinline__ uint4 load16(const int8_t *row, int at, int k) {
+    if (at + 16 <= k) return __ldg((const uint4 *)(row + at));
+    uint32_t v[4] = {0, 0, 0, 0};
+    for (int b = 0; b < 16 && at + b < k; b++) v[b >> 2] |= (uint32_t)(uint8_t)row[at + b] << (8 * (b & 3));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int MMA_WARPS = 8;
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearParams p) {
+    __shared__ int sums[MMA_WARPS][NT * 8][16];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int mtiles = (p.m + NT * 8 - 1) / (NT * 8);
+    const int m0 = (int)(blockIdx.x % mtiles) * NT * 8, n0 = (int)(blockIdx.x / mtiles) * 16;
+    // rows past the end repeat the last one; their sums are not stored
+    const int8_t *wa = p.w + (long long)min(n0 + g, p.n - 1) * p.w_stride;
+    const int8_t *wb = p.w + (long long)min(n0 + g + 8, p.n - 1) * p.w_stride;
+    const int8_t *xr[NT];
+    int acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        xr[j] = p.x + (long long)min(m0 + j * 8 + g, p.m - 1) * p.x_stride;
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[j][i] = 0;
+    }
+#pragma unroll 2
+    for (int kc = warp * 64; kc < p.k; kc += MMA_WARPS * 64) {
+        const int at = kc + t * 16;
+        const uint4 a = load16(wa, at, p.k), b = load16(wb, at, p.k);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const uint4 x = load16(xr[j], at, p.k);
+            mma_s8(acc[j], a.x, b.x, a.y, b.y, x.x, x.y);
+            mma_s8(acc[j], a.z, b.z, a.w, b.w, x.z, x.w);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        sums[warp][j * 8 + t * 2][g] = acc[j][0];
+        sums[warp][j * 8 + t * 2 + 1][g] = acc[j][1];
+        sums[warp][j * 8 + t * 2][g + 8] = acc[j][2];
+        sums[warp][j * 8 + t * 2 + 1][g + 8] = acc[j][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 8 * 16; i += blockDim.x) {
+        const int mi = i >> 4, ni = i & 15, m = m0 + mi, n = n0 + ni;
+        if (m >= p.m || n >= p.n) continue;
+        int s = 0;
+#pragma unroll
+        for (int w = 0; w < MMA_WARPS; w++) s += sums[w][mi][ni];
+        float v = (float)s * p.x_scale[m] * p.w_scale[n];
+        if (p.bias) v += p.bias[n];
+        ((T *)p.out)[m * p.out_stride + n] = from_float<T>(v);
+    }
+}
+
+template <typename T> int launch_mma(const LinearParams &p, cudaStream_t s) {
+    const int nt = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
+    const long long grid = (long long)((p.m + nt * 8 - 1) / (nt * 8)) * ((p.n + 15) / 16);
+    if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
+    if (nt == 1) linear_int8_mma_kernel<T, 1><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
+    else if (nt == 2) linear_int8_mma_kernel<T, 2><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
+    else linear_int8_mma_kernel<T, 4><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
+    GEO_CUDA_CHECK(cudaGetLastError());
+    return GEO_SC_OK;
+}
+
+}  // namespace
+}  // namespace geo
+
+using namespace geo;
+
+extern "C" int geo_sc_linear_int8(int m, int n, int k, const int8_t *x, long long x_stride, const float *x_scale, const int8_t *w,
+                                  long long w_stride, const float *w_scale, const float *bias, int dtype, void *out,
+                                  long long out_stride, void *stream) {
+    if (m < 0 || n < 1 || k < 1) return fail(GEO_SC_ERR_SHAPE, "product of [%d, %d] and [%d, %d]", m, k, n, k);
+    if (k > 131071) return fail(GEO_SC_ERR_TOO_LARGE, "k = %d: sums of more than 131071 products may leave 32 bits", k);
+    if (!dtype_known(dtype)) return fail(GEO_SC_ERR_UNSUPPORTED, "unknown element type %d", dtype);
+    if (m == 0) return GEO_SC_OK;
+    if (!x || !x_scale || !w || !w_scale || !out) return fail(GEO_SC_ERR_NULL, "x, w, their scales and out are required");
+    if (x_stride < k || w_stride < k || out_stride < n) return fail(GEO_SC_ERR_SHAPE, "bad row stride");
+    if (!aligned_to(x, 16) || !aligned_to(w, 16) || x_stride % 16 || w_stride % 16)
+        return fail(GEO_SC_ERR_UNSUPPORTED, "rows of x and w have to start on 16-byte boundaries");
+    LinearParams p{x, w, x_scale, w_scale, bias, out, x_stride, w_stride, out_stride, m, n, k};
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == GEO_SC_DTYPE_F32) return launch_mma<float>(p, s);
+    if (dtype == GEO_SC_DTYPE_BF16) return launch_mma<__nv_bfloat16>(p, s);
+    return launch_mma<__half>(p, s);
+}

@@ -259,3 +259,79 @@ def sc_block(conv, bn, x, conv_kwargs, next_conv, next_kwargs, astreams=None, pr
                               next_conv.kernel_size[0], next_conv.kernel_size[1], nsc.pop("bit_length"), nsc.pop("mode"), **nsc)
     return _SCBlock.apply(x, conv.weight, bn.weight if bn.affine else None, bn.bias if bn.affine else None, bn, sc,
                           next_desc, cache, astreams)
+
+
+class RMSNorm_Int8(nn.Module):
+    """Root-mean-square norm whose output are 8-bit integers with a scale per row, for evaluation
+    (:func:`geo_b200.functional.rms_norm_int8`): ``forward(x, residual=None)`` returns ``(q, scale)`` or
+    ``(q, scale, x + residual)``, the pair as :class:`Linear_Int8` takes it."""
+
+    def __init__(self, features, eps=1e-6):
+        super().__init__()
+        self.eps = float(eps)
+        self.register_buffer("weight", torch.ones(features))
+
+    @classmethod
+    def from_float(cls, norm):
+        """From an ``nn.RMSNorm`` over the last dimension."""
+        if len(norm.normalized_shape) != 1:
+            raise ValueError(f"only norms over the last dimension, got normalized_shape {tuple(norm.normalized_shape)}")
+        eps = norm.eps
+        if eps is None:     # nn.RMSNorm's default: the epsilon of the input's dtype, here of the weight's
+            eps = torch.finfo(norm.weight.dtype if norm.weight is not None else torch.float32).eps
+        new = cls(norm.normalized_shape[0], eps)
+        if norm.weight is not None:
+            new.weight = norm.weight.detach().clone()
+        return new
+
+    def forward(self, x, residual=None):
+        return sc_f.rms_norm_int8(x, self.weight, residual, self.eps)
+
+
+class Linear_Int8(nn.Module):
+    """Linear layer on 8-bit integers, for evaluation: weights with a scale per output channel, laid out once when the
+    layer is made, inputs with a scale per row (:func:`geo_b200.functional.linear_int8`).  The fixed-point counterpart
+    of :class:`Linear_Or`.  ``forward`` takes floating-point rows (quantised here) or the pair ``(q, scale)`` of
+    :class:`RMSNorm_Int8`; the output has the input's dtype, that of ``dtype`` for a pair (default float32)."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        super().__init__()
+        self.in_features, self.out_features = int(in_features), int(out_features)
+        # rows padded to 16 bytes: what the product reads without a copy
+        self.register_buffer("weight_q", torch.zeros(self.out_features, (self.in_features + 15) // 16 * 16, dtype=torch.int8))
+        self.register_buffer("weight_scale", torch.zeros(self.out_features))
+        self.register_buffer("bias", torch.zeros(self.out_features) if bias else None)
+
+    @classmethod
+    def from_float(cls, linear):
+        """From an ``nn.Linear`` or a :class:`Linear_Or` (its full-precision ``weight_org``) on a CUDA device."""
+        weight = getattr(linear, "weight_org", linear.weight).detach()
+        new = cls(linear.in_features, linear.out_features, linear.bias is not None).to(weight.device)
+        q, scale = sc_f.quantize_int8(weight)
+        new.weight_q[:, : new.in_features] = q
+        new.weight_scale.copy_(scale)
+        if linear.bias is not None:
+            new.bias.copy_(linear.bias.detach())
+        return new
+
+    def forward(self, input, dtype=None):
+        if isinstance(input, tuple):
+            q, scale = input
+            dtype = torch.float32 if dtype is None else dtype
+        else:
+            q, scale = sc_f.quantize_int8(input)
+            dtype = input.dtype if dtype is None else dtype
+        return sc_f.linear_int8(q, scale, self.weight_q[:, : self.in_features], self.weight_scale, self.bias, dtype)
+
+
+class DistillationLoss(nn.Module):
+    """:func:`geo_b200.functional.distillation_loss` with its settings kept: ``forward(logits, indices, teacher_logits,
+    weight=None, scale=1.0)``; ``scale`` multiplies the module's own."""
+
+    def __init__(self, temperature=1.0, reduction="batchmean", scale=1.0):
+        super().__init__()
+        self.temperature, self.reduction, self.scale = float(temperature), reduction, float(scale)
+
+    def forward(self, logits, indices, teacher_logits, weight=None, scale=1.0):
+        return sc_f.distillation_loss(logits, indices, teacher_logits, self.temperature, weight, self.reduction,
+                                      self.scale * scale)

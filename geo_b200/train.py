@@ -25,11 +25,18 @@ class TrainStep:
       step, as an eager call does;
     * the learning rate is read from a device scalar that is refreshed from
       ``optimizer.param_groups[0]['lr']`` before every replay, so schedulers keep working (SGD: the
-      update is written out with that scalar; Adam is built with ``capturable=True`` and a tensor lr)."""
+      update is written out with that scalar; Adam is built with ``capturable=True`` and a tensor lr).
 
-    def __init__(self, model, lr=2e-3, optim="SGD", grad_hook=None, graph=False):
+    ``distillation`` (a :class:`geo_b200.layers.DistillationLoss` with a scalar reduction) adds its loss to the cross
+    entropy, under the same loss scale; every call then takes ``teacher=(indices, logits)``, the teacher's top entries
+    for that batch (``torch.topk`` of its logits)."""
+
+    def __init__(self, model, lr=2e-3, optim="SGD", grad_hook=None, graph=False, distillation=None):
         self.model = model
         self.criterion = nn.CrossEntropyLoss()
+        if distillation is not None and distillation.reduction == "none":
+            raise ValueError("the distillation loss of a training step needs a scalar reduction")
+        self.distillation = distillation
         self.param_copy = [p.clone().float().detach().requires_grad_(True) for p in model.parameters()]
         if optim == "SGD":      # main_conv.py:216-217
             self.optimizer = torch.optim.SGD(self.param_copy, lr=lr, weight_decay=0, momentum=0.01)
@@ -55,12 +62,20 @@ class TrainStep:
         self._lr_dev = None       # graph mode, SGD: the learning rate the captured update reads
         self._captured = False    # inside graph capture or its warm-up: SGD update written out
 
-    def __call__(self, inputs, targets):
+    def __call__(self, inputs, targets, teacher=None):
+        if (teacher is None) != (self.distillation is None):
+            raise ValueError("teacher=(indices, logits) and a step made with distillation= come together")
         if not self.use_graph:
-            return self._step(inputs, targets)
+            return self._step(inputs, targets, teacher)
         if self._graph is None:
-            self._capture(inputs, targets)
-        sx, sy, sloss, sout = self._static
+            self._capture(inputs, targets, teacher)
+        sx, sy, steacher, sloss, sout = self._static
+        if steacher is not None:
+            for static, now in zip(steacher, teacher):
+                if static.shape != now.shape or static.dtype != now.dtype:
+                    raise ValueError(f"graph=True: the teacher's entries were {static.dtype} {tuple(static.shape)} at capture, "
+                                     f"now {now.dtype} {tuple(now.shape)}")
+                static.copy_(now, non_blocking=True)
         sx.copy_(inputs, non_blocking=True)
         sy.copy_(targets, non_blocking=True)
         self._refresh_lr()
@@ -103,8 +118,9 @@ class TrainStep:
                     if torch.is_tensor(v):
                         v.zero_()
 
-    def _capture(self, inputs, targets):
+    def _capture(self, inputs, targets, teacher=None):
         sx, sy = inputs.detach().clone(), targets.detach().clone()
+        steacher = tuple(t.detach().clone() for t in teacher) if teacher is not None else None
         if isinstance(self.optimizer, torch.optim.SGD):
             self._lr_host = float(self.optimizer.param_groups[0]["lr"])
             self._lr_dev = torch.full((), self._lr_host, dtype=torch.float32, device=sx.device)
@@ -114,7 +130,7 @@ class TrainStep:
         side.wait_stream(torch.cuda.current_stream(sx.device))
         with torch.cuda.stream(side):
             for _ in range(3):  # warm-up: lazy initialisation, optimiser state, allocator pools
-                self._step(sx.clone(), sy)
+                self._step(sx.clone(), sy, steacher)
         torch.cuda.current_stream(sx.device).wait_stream(side)
         torch.cuda.synchronize(sx.device)
         self._restore(snap)     # the warm-up steps must not count as training
@@ -122,13 +138,13 @@ class TrainStep:
         self._graph_update = None
         if self.grad_hook is None:
             with torch.cuda.graph(graph):
-                sloss, sout = self._step(sx.clone(), sy)
+                sloss, sout = self._step(sx.clone(), sy, steacher)
         else:
             # a hook that offers pack / reduce / unpack keeps its copies inside the graphs
             hook = self.grad_hook
             self._split_hook = all(hasattr(hook, n) for n in ("pack", "reduce", "unpack"))
             with torch.cuda.graph(graph):
-                sloss, sout = self._forward_backward(sx.clone(), sy)
+                sloss, sout = self._forward_backward(sx.clone(), sy, steacher)
                 if self._split_hook:
                     hook.pack(self.params)
             if self._split_hook:
@@ -142,20 +158,22 @@ class TrainStep:
                 self._update()
             self._graph_update = update
         self._graph = graph
-        self._static = (sx, sy, sloss, sout)
+        self._static = (sx, sy, steacher, sloss, sout)
 
-    def _step(self, inputs, targets):
-        out = self._forward_backward(inputs, targets)
+    def _step(self, inputs, targets, teacher=None):
+        out = self._forward_backward(inputs, targets, teacher)
         if self.grad_hook is not None:
             self.grad_hook(self.params)
         self._update()
         return out
 
-    def _forward_backward(self, inputs, targets):
+    def _forward_backward(self, inputs, targets, teacher=None):
         model = self.model
         model.train()
         output = model(inputs)
         loss = self.criterion(output, targets) * SCALE_FACTOR
+        if teacher is not None:
+            loss = loss + self.distillation(output, *teacher, scale=SCALE_FACTOR)
         for p in self.params:
             p.grad = None
         loss.backward()

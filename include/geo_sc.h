@@ -343,6 +343,65 @@ int geo_sc_pool_act_forward(int planes, int height, int width, const float *x_de
 int geo_sc_pool_act_backward(int planes, int height, int width, const float *x_device, const float *grad_y_device,
                              float *grad_x_device, void *stream);
 
+/* ---- 8-bit integers with one scale per row ---------------------------------------------------------
+ * The ordinary fixed-point counterpart of the SC layers, for evaluation: symmetric 8-bit integers, a scale per
+ * token and per output channel, exact integer sums.  No counterpart in the reference, whose fixed point has one
+ * range for a whole tensor (quantize, utils_functional.py:33-39; quantize_shift, :41-57).
+ *
+ * Floating-point tensors are of one of the types below; strides count elements, rows are dense. */
+#define GEO_SC_DTYPE_F32 0
+#define GEO_SC_DTYPE_BF16 1
+#define GEO_SC_DTYPE_F16 2
+
+/* Root-mean-square norm of each row, as 8-bit integers: r = x + residual rounded to the tensors' type (r = x without
+ * a residual), p = r * weight in fp32, q = round_half_even(127 p / max|p|), scale = max|p| / (127 * sqrt(mean(r^2) + eps)),
+ * so that q * scale is the normalised row.  q depends on the row alone, not on how it is summed.  residual and
+ * sum_out ([rows][cols] dense, receives r; it must not overlap x or residual) come together or are both NULL; weight
+ * [cols] of weight_dtype.  A row of zeros has q = 0 and scale = 0; a row whose p or scale is not finite has q = 0 and
+ * scale = NaN.  eps >= 0. */
+int geo_sc_rms_norm_int8(long long rows, int cols, int dtype, const void *x_device, long long x_stride,
+                         const void *residual_device, long long residual_stride, const void *weight_device,
+                         int weight_dtype, float eps, void *sum_out_device, int8_t *q_device, long long q_stride,
+                         float *scale_device, void *stream);
+
+/* The same integers without the norm: q = round_half_even(127 x / max|x|), scale = max|x| / 127 (rows of tokens, and
+ * rows of weights with one scale per output channel). */
+int geo_sc_quantize_int8(long long rows, int cols, int dtype, const void *x_device, long long x_stride, int8_t *q_device,
+                         long long q_stride, float *scale_device, void *stream);
+
+/* out[row][col] = q * scale[row], rounded once to dtype; out is [rows][cols] dense. */
+int geo_sc_dequantize_int8(long long rows, int cols, const int8_t *q_device, long long q_stride, const float *scale_device,
+                           int dtype, void *out_device, void *stream);
+
+/* out[i][j] = (sum_k x[i][k] w[j][k]) * x_scale[i] * w_scale[j] + bias[j]: the integer sum is exact, scales and bias are
+ * fp32, one rounding to dtype.  x [m][k] and w [n][k] int8 with rows that start on 16-byte boundaries (base and strides
+ * multiples of 16; GEO_SC_ERR_UNSUPPORTED otherwise), k <= 131071; bias [n] fp32 or NULL. */
+int geo_sc_linear_int8(int m, int n, int k, const int8_t *x_device, long long x_stride, const float *x_scale_device,
+                       const int8_t *w_device, long long w_stride, const float *w_scale_device, const float *bias_device,
+                       int dtype, void *out_device, long long out_stride, void *stream);
+
+/* ---- distillation from a teacher's top logits --------------------------------------------------------
+ * Beside the cross entropy of the reference's training loop (utils_own.py:57-114), which knows class labels only.
+ * logits [rows][vocab] of dtype, indices [rows][top] of index_bits (32 or 64) and teacher [rows][top] of teacher_dtype
+ * dense, weight [rows] fp32 or NULL (all 1), top <= 512.  Per row, with p the softmax over the entries of teacher / T
+ * and q the softmax over the vocabulary of logits / T:
+ *     row loss = weight * T^2 * sum_k p_k (log p_k - log q[index_k])
+ * Entries with a negative index are padding.  A row of weight 0 or without an entry above -inf has loss 0 and gradient
+ * 0; an index >= vocab or a teacher's logit that is NaN or +inf gives the row a loss and a gradient of NaN.
+ * mean != 0: loss[0] = scale * (sum of the row losses) / rows (0 rows: 0), added in a fixed order; row_loss [rows]
+ * receives the unscaled row losses.  mean == 0: row_loss receives scale * row loss.  stats: 8 bytes per row for the
+ * backward pass.  grad ([rows][vocab] dense, or NULL): the gradient for an upstream gradient of 1. */
+int geo_sc_distill_forward(long long rows, int vocab, int top, int dtype, const void *logits_device, long long stride,
+                           const void *indices_device, int index_bits, const void *teacher_device, int teacher_dtype,
+                           const float *weight_device, float temperature, float scale, int mean, float *row_loss_device,
+                           void *stats_device, float *loss_device, void *grad_device, void *stream);
+/* Gradient for upstream ([1] if mean, else [rows]; fp32, device).  skip_one != 0: grad already holds the forward
+ * pass's gradient, and rows whose upstream gradient is exactly 1 are left as they are. */
+int geo_sc_distill_backward(long long rows, int vocab, int top, int dtype, const void *logits_device, long long stride,
+                            const void *indices_device, int index_bits, const void *teacher_device, int teacher_dtype,
+                            const float *weight_device, float temperature, float scale, int mean, const void *stats_device,
+                            const float *upstream_device, int skip_one, void *grad_device, void *stream);
+
 /* ---- host mirror of the stream generator ------------------------------------------------
  * Runs on the CPU with the same pattern tables and loading plan the kernels use, for one
  * integer level `value` in [0, bit_length): seed = (seed_base + seed_index) mod (L-1) + 1
