@@ -5,6 +5,7 @@ There is no fallback: if the library is missing or a call fails, an exception is
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -33,6 +34,24 @@ GENERATORS = {"lfsr": 0, "acc": 1, "rand": 2}
 
 
 _lib = None
+_rows = None
+
+
+def rows():
+    """Load ``ext/geo_rows.so``: the torch front end of the 8-bit row operators and of the distillation loss."""
+    global _rows
+    if _rows is None:
+        path = os.path.join(PKG, "ext", "geo_rows.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: run `python -m geo_b200.build` (there is no fallback path)")
+        import torch  # noqa: F401  (libtorch before the extension module)
+
+        lib()
+        spec = importlib.util.spec_from_file_location("geo_rows", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _rows = module
+    return _rows
 
 
 def lib():

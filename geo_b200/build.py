@@ -18,7 +18,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libgeo_sc.so")
-EXT_DIR = os.path.join(PKG, "ext")  # holds sc_extension_cuda*.so and sc_extension*.so
+EXT_DIR = os.path.join(PKG, "ext")  # holds sc_extension_cuda.so, sc_extension.so and geo_rows.so
 
 CUDA_SOURCES = ["sc_api.cu", "sc_streams.cu", "sc_accumulate.cu", "sc_accumulate_sorted.cu", "sc_accumulate_rows.cu", "sc_accumulate_taps.cu", "sc_accumulate_short.cu", "sc_accumulate_fullbin.cu", "sc_peak.cu", "sc_guide.cu", "sc_guide_mma.cu", "sc_guide_tc.cu", "sc_bn.cu", "sc_static.cu", "sc_norm_int8.cu", "sc_linear_int8.cu", "sc_distill.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -82,8 +82,8 @@ def build_lib(force=False, verbose=False, ptxas_info=False):
 
 
 def build_torch_ext(force=False, verbose=False):
-    """g++ -> geo_b200/ext/sc_extension_cuda.so and geo_b200/ext/sc_extension.so (pybind11 shims
-    over the C ABI; no CUDA code of their own)."""
+    """g++ -> geo_b200/ext/sc_extension_cuda.so, geo_b200/ext/sc_extension.so and geo_b200/ext/geo_rows.so
+    (pybind11 shims over the C ABI; no CUDA code of their own)."""
     import torch
     from torch.utils import cpp_extension as ce
 
@@ -101,8 +101,8 @@ def build_torch_ext(force=False, verbose=False):
     link = [f"-L{libdir}", f"-Wl,-rpath,{libdir}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_cuda",
             "-ltorch_python", f"-L{LIB_DIR}", "-lgeo_sc", "-Wl,-rpath,$ORIGIN/../lib"]
     out = []
-    for name in ("sc_extension_cuda", "sc_extension"):
-        src = os.path.join(CSRC, name + ".cpp")
+    for name, file in (("sc_extension_cuda", "sc_extension_cuda"), ("sc_extension", "sc_extension"), ("geo_rows", "sc_rows_extension")):
+        src = os.path.join(CSRC, file + ".cpp")
         target = os.path.join(EXT_DIR, name + ".so")
         out.append(target)
         if not force and not _stale(target, [src, os.path.join(ROOT, "include", "geo_sc.h")]):

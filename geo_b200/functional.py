@@ -168,11 +168,6 @@ def sc_forward_counts(activation, weight, bit_length, forward="1d_bin", padding=
 # ---- 8-bit integers with one scale per row: the fixed-point counterpart of the SC layers, for evaluation ----
 
 
-def _evaluation_only(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient (evaluation only): call it under torch.no_grad() or detach its inputs")
-
-
 def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     """Root-mean-square norm over the last dimension as 8-bit integers with one scale per row.
 
@@ -181,14 +176,12 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     ``q * scale`` is the normalised row.  Returns ``(q, scale)``, or ``(q, scale, r)`` when a residual is given.
     ``x`` float32, bfloat16 or float16, any leading dimensions; ``weight`` of any of these types.  A row of zeros has
     scale 0; a row that holds an infinity or a NaN has q = 0 and scale = NaN.  Evaluation only, CUDA tensors only."""
-    _evaluation_only("rms_norm_int8", x, weight, residual)
     return ops.rms_norm_int8(x, weight, residual, eps)
 
 
 def quantize_int8(x):
     """``(q, scale)`` with ``q = round(127 x / max|x|)`` and ``scale = max|x| / 127`` over the last dimension: tokens
     with a scale each, or a weight ``[out, in]`` with a scale per output channel.  Evaluation only."""
-    _evaluation_only("quantize_int8", x)
     return ops.quantize_int8(x)
 
 
@@ -201,34 +194,10 @@ def linear_int8(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32
     """``(q @ weight_q.T) * scale[..., None] * weight_scale + bias`` for 8-bit integers ``q [..., k]`` with a scale per
     row and ``weight_q [n, k]`` with a scale per output channel: exact integer sums, one rounding to ``dtype``.
     ``k`` up to 131071.  Evaluation only."""
-    _evaluation_only("linear_int8", scale, weight_scale, bias)
     return ops.linear_int8(q, scale, weight_q, weight_scale, bias, dtype)
 
 
 # ---- training against a teacher ---------------------------------------------------------------------------
-
-
-class _Distillation(torch.autograd.Function):
-    """With a scalar loss the forward pass writes the gradient for an upstream gradient of 1 along with the loss (the
-    logits are read once); the backward pass hands it over, and writes it anew where the upstream gradient turns out
-    not to be 1 or where it runs a second time."""
-
-    @staticmethod
-    def forward(ctx, logits, indices, teacher_logits, weight, temperature, scale, mean):
-        loss, stats, ctx.ready = ops.distill_forward(logits, indices, teacher_logits, temperature, weight, scale, mean,
-                                                     need_grad=mean and ctx.needs_input_grad[0])
-        ctx.settings = (temperature, scale, mean)
-        ctx.save_for_backward(logits, indices, teacher_logits, weight, stats)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, upstream):
-        logits, indices, teacher_logits, weight, stats = ctx.saved_tensors
-        temperature, scale, mean = ctx.settings
-        ready, ctx.ready = ctx.ready, None
-        grad = ops.distill_backward(logits, indices, teacher_logits, stats, upstream, temperature, weight, scale, mean, ready)
-        return grad, None, None, None, None, None, None
 
 
 def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=None, reduction="batchmean", scale=1.0):
@@ -245,11 +214,4 @@ def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=N
 
     ``scale`` is part of the loss; a loss scale or the loss's share in a sum is best given here, because the gradient
     is computed along with the loss for an upstream gradient of 1 and again where that turns out to be another."""
-    if reduction not in ("batchmean", "sum", "none"):
-        raise ValueError(f"reduction must be 'batchmean', 'sum' or 'none', got {reduction!r}")
-    if torch.is_grad_enabled() and (teacher_logits.requires_grad or (weight is not None and weight.requires_grad)):
-        raise ValueError("distillation_loss has no gradient for teacher_logits and weight: detach them")
-    scale = float(scale)
-    if reduction == "sum":     # the kernels divide by the number of rows
-        scale *= max(1, logits.shape[:-1].numel())
-    return _Distillation.apply(logits, indices, teacher_logits, weight, float(temperature), scale, reduction != "none")
+    return ops.distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)

@@ -321,7 +321,10 @@ class Linear_Int8(nn.Module):
         else:
             q, scale = sc_f.quantize_int8(input)
             dtype = input.dtype if dtype is None else dtype
-        return sc_f.linear_int8(q, scale, self.weight_q[:, : self.in_features], self.weight_scale, self.bias, dtype)
+        w = self.weight_q
+        if w.shape[1] != self.in_features:
+            w = w[:, : self.in_features]
+        return sc_f.linear_int8(q, scale, w, self.weight_scale, self.bias, dtype)
 
 
 class DistillationLoss(nn.Module):

@@ -19,9 +19,21 @@ class _Stats:
     on the launching stream and recorded as (algorithmic LOP3 count, algorithmic bytes, start, end)."""
 
     def __init__(self):
-        self.launches = 0
+        self._count = 0      # beside what the C++ front end counts by itself
         self.profile = False
         self.records = []
+
+    @staticmethod
+    def _counted_in_cpp():
+        return _lib._rows.launches() if _lib._rows is not None else 0
+
+    @property
+    def launches(self):
+        return self._count + self._counted_in_cpp()
+
+    @launches.setter
+    def launches(self, value):
+        self._count = value - self._counted_in_cpp()
 
     def reset(self):
         self.launches = 0
@@ -470,215 +482,31 @@ def epilogue_backward(counts, in_bit_length, grad_out, weight, mean, invstd, wq,
     return gx, gw, gb
 
 
-# ---- 8-bit integers with one scale per row, and the distillation loss ------------------------------------
-
-_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _dtype_code(dtype, what):
-    code = _DTYPE_CODE.get(dtype)
-    if code is None:
-        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {dtype}")
-    return code
-
-
-def _require_one_device(*tensors):
-    tensors = [t for t in tensors if t is not None]
-    _require_cuda(*tensors)
-    for t in tensors:
-        if t.device != tensors[0].device:
-            raise ValueError(f"tensors on {tensors[0].device} and {t.device} in one call")
-
-
-def _rows_of(t):
-    """``t`` as [rows, last dimension] with dense rows (a view where the strides allow one)."""
-    r = t.detach()
-    if r.dim() != 2:
-        r = r.reshape(-1, r.shape[-1])
-    return r if r.stride(1) == 1 or r.shape[1] == 1 else r.contiguous()
-
-
-def empty_int8_rows(rows, cols, device):
-    """An int8 tensor [rows, cols] whose rows start on 16-byte boundaries, as :func:`linear_int8` reads them."""
-    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :cols]
-
-
-def _aligned_int8(t):
-    """``t`` itself if its rows start on 16-byte boundaries, else a copy whose rows do."""
-    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    return empty_int8_rows(t.shape[0], t.shape[1], t.device).copy_(t)
-
-
-def _check_row_operand(x, what):
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{what} needs a last dimension of at least 1, got shape {tuple(x.shape)}")
-    if max(x.shape[-1], x.numel() // x.shape[-1]) > 0x7fffffff:
-        raise ValueError(f"{what} has more than 2^31 - 1 rows or columns: {tuple(x.shape)}")
+# ---- 8-bit integers with one scale per row, and the distillation loss (checks and launches in C++: _lib.rows) ----
 
 
 def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     """Root-mean-square norm of the rows of ``x`` (plus ``residual``) as 8-bit integers -> (q, scale) or, with a
     residual, (q, scale, x + residual); shapes [..., cols], [...], [..., cols]."""
-    code = _dtype_code(x.dtype, "x")
-    wcode = _dtype_code(weight.dtype, "weight")
-    _check_row_operand(x, "x")
-    cols = x.shape[-1]
-    if tuple(weight.shape) != (cols,):
-        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({cols},)")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"residual is {residual.dtype} {tuple(residual.shape)}, x is {x.dtype} {tuple(x.shape)}")
-    eps = float(eps)
-    if not 0.0 <= eps < 3.4e38:
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
-    _require_one_device(x, weight, residual)
-    xr, w = _rows_of(x), weight.detach().contiguous()
-    rr = _rows_of(residual) if residual is not None else None
-    rows, dev = xr.shape[0], x.device
-    with torch.cuda.device(dev):
-        q = empty_int8_rows(rows, cols, dev)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        total = torch.empty(x.shape, dtype=x.dtype, device=dev) if rr is not None else None
-        check(_lib.lib().geo_sc_rms_norm_int8(rows, cols, code, xr.data_ptr(), xr.stride(0), _ptr(rr),
-                                              rr.stride(0) if rr is not None else 0, w.data_ptr(), wcode, eps, _ptr(total),
-                                              q.data_ptr(), q.stride(0), scale.data_ptr(), _stream_ptr(dev)),
-              "geo_sc_rms_norm_int8")
-    STATS.launches += 1 if rows else 0
-    q = q if x.dim() == 2 else q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0]
-    return (q, scale) if rr is None else (q, scale, total)
+    return _lib.rows().rms_norm_int8(x, weight, residual, eps)
 
 
 def quantize_int8(x):
     """Rows of ``x`` as 8-bit integers with one scale per row -> (q [..., cols], scale [...])."""
-    code = _dtype_code(x.dtype, "x")
-    _check_row_operand(x, "x")
-    _require_one_device(x)
-    xr = _rows_of(x)
-    rows, cols = xr.shape
-    dev = x.device
-    with torch.cuda.device(dev):
-        q = empty_int8_rows(rows, cols, dev)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        check(_lib.lib().geo_sc_quantize_int8(rows, cols, code, xr.data_ptr(), xr.stride(0), q.data_ptr(), q.stride(0),
-                                              scale.data_ptr(), _stream_ptr(dev)), "geo_sc_quantize_int8")
-    STATS.launches += 1 if rows else 0
-    q = q if x.dim() == 2 else q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0]
-    return q, scale
+    return _lib.rows().quantize_int8(x)
 
 
 def dequantize_int8(q, scale, dtype=torch.float32):
     """``q * scale`` per row, rounded once to ``dtype``."""
-    code = _dtype_code(dtype, "dtype")
-    if q.dtype != torch.int8 or scale.dtype != torch.float32:
-        raise TypeError(f"q must be int8 and scale float32, got {q.dtype} and {scale.dtype}")
-    _check_row_operand(q, "q")
-    if scale.shape != q.shape[:-1]:
-        raise ValueError(f"scale has shape {tuple(scale.shape)}, expected {tuple(q.shape[:-1])}")
-    _require_one_device(q, scale)
-    qr, s = _rows_of(q), scale.detach().contiguous()
-    dev = q.device
-    with torch.cuda.device(dev):
-        out = torch.empty(q.shape, dtype=dtype, device=dev)
-        check(_lib.lib().geo_sc_dequantize_int8(qr.shape[0], qr.shape[1], qr.data_ptr(), qr.stride(0), s.data_ptr(), code,
-                                                out.data_ptr(), _stream_ptr(dev)), "geo_sc_dequantize_int8")
-    STATS.launches += 1 if qr.shape[0] else 0
-    return out
+    return _lib.rows().dequantize_int8(q, scale, dtype)
 
 
 def linear_int8(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32):
     """8-bit matrix product [..., k] x [n, k] -> [..., n] with a scale per row of either operand.  Operands whose rows
     do not start on 16-byte boundaries are copied first (the quantisers of this module leave rows that do)."""
-    code = _dtype_code(dtype, "dtype")
-    if q.dtype != torch.int8 or weight_q.dtype != torch.int8:
-        raise TypeError(f"the operands must be int8, got {q.dtype} and {weight_q.dtype}")
-    if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32 or (bias is not None and bias.dtype != torch.float32):
-        raise TypeError("scales and bias must be float32")
-    _check_row_operand(q, "q")
-    if weight_q.dim() != 2 or weight_q.shape[0] < 1 or weight_q.shape[1] != q.shape[-1]:
-        raise ValueError(f"feature mismatch: q is {tuple(q.shape)}, weight {tuple(weight_q.shape)}")
-    n, k = weight_q.shape
-    if scale.shape != q.shape[:-1] or tuple(weight_scale.shape) != (n,) or (bias is not None and tuple(bias.shape) != (n,)):
-        raise ValueError(f"scales {tuple(scale.shape)}, {tuple(weight_scale.shape)} and bias do not match rows of "
-                         f"{tuple(q.shape)} and {tuple(weight_q.shape)}")
-    if k > 131071:
-        raise ValueError(f"k = {k}: sums of more than 131071 products may leave 32 bits")
-    _require_one_device(q, scale, weight_q, weight_scale, bias)
-    dev = q.device
-    with torch.cuda.device(dev):
-        x, w = _aligned_int8(_rows_of(q)), _aligned_int8(weight_q.detach())
-        s, ws = scale.detach().contiguous(), weight_scale.detach().contiguous()
-        b = bias.detach().contiguous() if bias is not None else None
-        m = x.shape[0]
-        out = torch.empty((*q.shape[:-1], n), dtype=dtype, device=dev)
-        check(_lib.lib().geo_sc_linear_int8(m, n, k, x.data_ptr(), x.stride(0), s.data_ptr(), w.data_ptr(), w.stride(0),
-                                            ws.data_ptr(), _ptr(b), code, out.data_ptr(), n, _stream_ptr(dev)),
-              "geo_sc_linear_int8")
-    STATS.launches += 1 if m else 0
-    return out
+    return _lib.rows().linear_int8(q, scale, weight_q, weight_scale, bias, dtype)
 
 
-def _distill_operands(logits, indices, teacher_logits, temperature, weight, scale):
-    code, tcode = _dtype_code(logits.dtype, "logits"), _dtype_code(teacher_logits.dtype, "teacher_logits")
-    if indices.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"indices must be int64 or int32, got {indices.dtype}")
-    _check_row_operand(logits, "logits")
-    if indices.shape != teacher_logits.shape or indices.shape[:-1] != logits.shape[:-1] or indices.dim() != logits.dim():
-        raise ValueError(f"logits {tuple(logits.shape)}, indices {tuple(indices.shape)} and teacher_logits "
-                         f"{tuple(teacher_logits.shape)} do not match")
-    if not 1 <= indices.shape[-1] <= 512:
-        raise ValueError(f"between 1 and 512 entries per row, got {indices.shape[-1]}")
-    if weight is not None and (weight.shape != logits.shape[:-1] or weight.dtype != torch.float32):
-        raise ValueError(f"weight must be float32 of shape {tuple(logits.shape[:-1])}, got {weight.dtype} {tuple(weight.shape)}")
-    if not 1e-6 <= float(temperature) <= 1e6:
-        raise ValueError(f"temperature must lie in [1e-6, 1e6], got {temperature}")
-    if not abs(float(scale)) < float("inf"):
-        raise ValueError(f"scale must be finite, got {scale}")
-    _require_one_device(logits, indices, teacher_logits, weight)
-    z = _rows_of(logits)
-    idx, t = indices.detach().contiguous(), teacher_logits.detach().contiguous()
-    w = weight.detach().contiguous() if weight is not None else None
-    return z, idx, t, w, code, tcode
-
-
-def distill_forward(logits, indices, teacher_logits, temperature=1.0, weight=None, scale=1.0, mean=True, need_grad=False):
-    """Distillation loss -> (loss, stats, grad): loss a scalar (``mean``) or one value per row, stats what
-    :func:`distill_backward` needs, grad the gradient for an upstream gradient of 1 (None unless ``need_grad``)."""
-    z, idx, t, w, code, tcode = _distill_operands(logits, indices, teacher_logits, temperature, weight, scale)
-    rows, vocab = z.shape
-    dev = logits.device
-    with torch.cuda.device(dev):
-        row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if mean else None
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if need_grad else None
-        check(_lib.lib().geo_sc_distill_forward(rows, vocab, idx.shape[-1], code, z.data_ptr(), z.stride(0), idx.data_ptr(),
-                                                64 if idx.dtype == torch.int64 else 32, t.data_ptr(), tcode, _ptr(w),
-                                                float(temperature), float(scale), int(bool(mean)), row_loss.data_ptr(),
-                                                stats.data_ptr(), _ptr(loss), _ptr(grad), _stream_ptr(dev)),
-              "geo_sc_distill_forward")
-    STATS.launches += (1 if rows else 0) + (1 if mean else 0)
-    return (loss if mean else row_loss), stats, grad
-
-
-def distill_backward(logits, indices, teacher_logits, stats, upstream, temperature=1.0, weight=None, scale=1.0, mean=True,
-                     grad=None):
-    """Gradient of :func:`distill_forward` for ``upstream`` (a scalar if ``mean``, else one value per row).  ``grad``: the
-    gradient that the forward pass has written; it is kept where the upstream gradient is exactly 1 and written anew
-    where it is not (decided on the device)."""
-    z, idx, t, w, code, tcode = _distill_operands(logits, indices, teacher_logits, temperature, weight, scale)
-    rows, vocab = z.shape
-    dev = logits.device
-    with torch.cuda.device(dev):
-        up = upstream.detach().to(torch.float32).contiguous()
-        if up.numel() != (1 if mean else rows):
-            raise ValueError(f"upstream has {up.numel()} values, expected {1 if mean else rows}")
-        have = grad is not None
-        if not have:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        check(_lib.lib().geo_sc_distill_backward(rows, vocab, idx.shape[-1], code, z.data_ptr(), z.stride(0), idx.data_ptr(),
-                                                 64 if idx.dtype == torch.int64 else 32, t.data_ptr(), tcode, _ptr(w),
-                                                 float(temperature), float(scale), int(bool(mean)), stats.data_ptr(),
-                                                 up.data_ptr(), int(have), grad.data_ptr(), _stream_ptr(dev)),
-              "geo_sc_distill_backward")
-    STATS.launches += 1 if rows else 0
-    return grad
+def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=None, reduction="batchmean", scale=1.0):
+    """Distillation loss, differentiable in ``logits``: a scalar, or one value per row for ``reduction='none'``."""
+    return _lib.rows().distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)

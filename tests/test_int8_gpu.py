@@ -118,7 +118,7 @@ def test_norm_strides_and_shapes(cuda_device, dtype):
         assert q.shape == x.shape and scale.shape == x.shape[:-1] and total.shape == x.shape
         check_norm(x, res, w, 1e-5, (q, scale, total))
         q, scale = F.quantize_int8(x)
-        assert torch.equal(q.cpu(), reference_rows(x.cpu(), None)[0])
+        assert torch.equal(q.cpu(), reference_rows(x.cpu(), None)[0]) and (q.dim() < 2 or q.stride(-2) % 16 == 0)
         y = F.dequantize_int8(q, scale, dtype)
         exact = q.cpu().double() * scale.cpu().double()[..., None]
         assert y.shape == x.shape and ((y.cpu().double() - exact).abs() <= exact.abs() * (half_step(dtype) + STEP32) + 2.0 ** -25).all()
@@ -143,9 +143,7 @@ def test_quantised_rows_do_not_depend_on_their_neighbours(cuda_device):
 
 
 def int8_rows(g, rows, cols, device, low=-128):
-    from geo_b200 import ops
-
-    t = ops.empty_int8_rows(rows, cols, device)
+    t = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :cols]
     return t.copy_(torch.randint(low, 128, (rows, cols), generator=g, dtype=torch.int8))
 
 

@@ -93,11 +93,15 @@ def test_training_step_and_its_teacher_come_together():
 
 
 def test_rows_for_the_product_are_padded():
-    q = ops.empty_int8_rows(3, 17, "cpu")
-    assert q.shape == (3, 17) and q.stride() == (32, 1)
-    q.fill_(1)
-    assert ops._aligned_int8(q) is q
-    copy = ops._aligned_int8(torch.ones(3, 17, dtype=torch.int8))
-    assert copy.stride(0) == 32 and torch.equal(copy, q)
-    layer = layers.Linear_Int8(17, 5)
-    assert layer.weight_q.shape == (5, 32)
+    assert layers.Linear_Int8(17, 5).weight_q.shape == (5, 32)
+    assert layers.Linear_Int8(32, 5).weight_q.shape == (5, 32)
+
+
+def test_launch_count_is_one_number():
+    stats = ops._Stats()
+    ops._lib.rows()
+    stats.reset()
+    stats.launches += 3
+    assert stats.launches == 3
+    stats.reset()
+    assert stats.launches == 0
