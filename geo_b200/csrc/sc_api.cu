@@ -6,6 +6,7 @@
 #include "sc_common.h"
 #include "sc_fullbin.h"
 #include "sc_guide_tc.h"
+#include "sc_linear_int8.h"
 #include "sc_rows.h"
 #include "sc_short.h"
 #include "sc_sorted.h"
@@ -239,7 +240,11 @@ int geo_sc_init(void) { return ensure_tables(); }
 
 int geo_sc_device_error_count(int *count) {
     if (!count) return fail(GEO_SC_ERR_NULL, "count is NULL");
-    return tc_error_count(count);
+    int guide = 0, linear = 0;
+    int rc = tc_error_count(&guide);
+    if (!rc) rc = linear_int8_tc_error_count(&linear);
+    if (!rc) *count = guide + linear;
+    return rc;
 }
 
 int geo_sc_group_geometry(const geo_sc_conv_desc *desc, int32_t *groups, int32_t *members, int32_t *members_padded,

@@ -5,22 +5,16 @@
 // The sum is exact in 32-bit integers (k <= 131071, so that 2^14 k stays below 2^31); the two scales and the bias are
 // applied in fp32 and the result is rounded once to the output's type.
 //
+// Up to 32 tokens run on linear_int8_mma_kernel below, more on the tcgen05 kernel (sc_linear_int8_tc.cu).
+//
 // linear_int8_mma_kernel: `mma.sync.m16n8k32` with the weights as the 16-row operand, read once from memory straight
 // into fragments.  The order of k inside a product is free, so a lane takes 16 consecutive bytes of its weight row and
 // the same 16 bytes of its token rows for two instructions: whole 16-byte loads, no shared memory, no shuffles.  A CTA
 // of eight warps owns 16 channels x 8 * NT tokens; the warps split k and join their integer sums in shared memory.
-#include "sc_rows8.h"
+#include "sc_linear_int8.h"
 
 namespace geo {
 namespace {
-
-struct LinearParams {
-    const int8_t *x, *w;
-    const float *x_scale, *w_scale, *bias;
-    void *out;
-    long long x_stride, w_stride, out_stride;
-    int m, n, k;
-};
 
 // 16 bytes of a row from byte `at` on, zeros from byte k on.
 __device__ __forceinline__ uint4 load16(const int8_t *row, int at, int k) {
@@ -107,6 +101,7 @@ extern "C" int geo_sc_linear_int8(int m, int n, int k, const int8_t *x, long lon
                                   long long out_stride, void *stream) {
     if (m < 0 || n < 1 || k < 1) return fail(GEO_SC_ERR_SHAPE, "product of [%d, %d] and [%d, %d]", m, k, n, k);
     if (k > 131071) return fail(GEO_SC_ERR_TOO_LARGE, "k = %d: sums of more than 131071 products may leave 32 bits", k);
+    if (m > 0x7ffffe00 || n > 0x7ffffe00) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", m, n);
     if (!dtype_known(dtype)) return fail(GEO_SC_ERR_UNSUPPORTED, "unknown element type %d", dtype);
     if (m == 0) return GEO_SC_OK;
     if (!x || !x_scale || !w || !w_scale || !out) return fail(GEO_SC_ERR_NULL, "x, w, their scales and out are required");
@@ -115,6 +110,7 @@ extern "C" int geo_sc_linear_int8(int m, int n, int k, const int8_t *x, long lon
         return fail(GEO_SC_ERR_UNSUPPORTED, "rows of x and w have to start on 16-byte boundaries");
     LinearParams p{x, w, x_scale, w_scale, bias, out, x_stride, w_stride, out_stride, m, n, k};
     cudaStream_t s = (cudaStream_t)stream;
+    if (m > 32) return launch_linear_int8_tc(p, dtype, s);
     if (dtype == GEO_SC_DTYPE_F32) return launch_mma<float>(p, s);
     if (dtype == GEO_SC_DTYPE_BF16) return launch_mma<__nv_bfloat16>(p, s);
     return launch_mma<__half>(p, s);

@@ -1,0 +1,347 @@
+// The 8-bit matrix product on the fifth-generation tensor cores: tcgen05.mma kind::i8, 32-bit integer accumulators in
+// tensor memory, operand tiles brought in by TMA (which fills rows and bytes past the end with zeros, so every size
+// takes the same path).
+//
+// The weights are the 128-lane operand: an accumulator's lane is an output channel and its columns are tokens, so that
+// the 32 lanes of a warp store 32 neighbouring channels of one token, for any n, and a lane keeps one weight scale and
+// one bias.  A tile is 128 channels x BN tokens of one CTA, or 256 channels x 256 tokens of a pair of CTAs
+// (cta_group::2): each of the pair loads its 128 channels and half of the tokens, the even CTA issues the
+// instructions for both, and each keeps the accumulators of its own channels.
+//
+// Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
+// out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the
+// CTA stops waiting, lets its own copies and instructions in flight finish (again with a bound) and leaves.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "sc_linear_int8.h"
+
+namespace geo {
+
+__device__ int g_linear_tc_errors = 0;
+
+namespace {
+
+constexpr int LT_THREADS = 320;
+constexpr int LT_EPI_WARPS = 8;
+constexpr int LT_KB = 128;                // bytes of k per stage: one 128-byte swizzled row
+constexpr int LT_SPIN_LIMIT = 1 << 22;
+
+template <int CTAS, int BN> struct LinearTile {
+    static constexpr int X_ROWS = BN / CTAS;                                  // token rows that a CTA loads
+    static constexpr int STAGE = (128 + X_ROWS) * LT_KB;
+    static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;    // at most 192 KB of tiles
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;          // two accumulators
+    // kind::i8: 32-bit integers out (2), signed 8-bit A and B (1), both K-major
+    static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CTAS * 128 >> 4) << 24);
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t rank0_address(uint32_t addr) {   // the same place in the pair's even CTA
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
+    return r;
+}
+template <int CTAS> __device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+    if (CTAS == 1) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(rank0_address(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+    for (int i = 0; i < LT_SPIN_LIMIT; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023) == 1023 && *abort) return false;
+    }
+    if (!*abort) {
+        *abort = 1;
+        atomicAdd(&g_linear_tc_errors, 1);
+    }
+    return false;
+}
+// After an abort: whatever is still in flight towards `bar` gets its time to arrive.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < LT_SPIN_LIMIT && !mbar_try_wait(bar, parity); i++) {}
+}
+
+template <int CTAS> __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+    if (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+                     : "memory");
+    else   // the barrier is the even CTA's
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+                     : "memory");
+}
+
+// Shared-memory matrix descriptor: K-major rows of 128 bytes under the 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if (CTAS == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+                     ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+                     ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+template <int CTAS> __device__ __forceinline__ void umma_commit(uint32_t bar) {   // on the barrier of every CTA of the tile
+    if (CTAS == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+                     ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+}
+template <int CTAS> __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+    if (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+}
+template <int CTAS> __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+    if (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+// The registers of the load above may be read from here on (they pass through, so that nothing that reads them moves up).
+__device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+template <int CTAS> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the pair
+    if (CTAS == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+
+template <typename T, int CTAS, int BN>
+__global__ void __launch_bounds__(LT_THREADS, 1)
+linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearParams pr, int ntiles_n, int ntiles) {
+    using Tile = LinearTile<CTAS, BN>;
+    constexpr int ST = Tile::STAGES;
+    extern __shared__ unsigned char lt_smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * ST + 5];   // full, empty, acc_full[2], acc_empty[2], drain
+    __shared__ __align__(16) float scales[LT_EPI_WARPS][16];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const uint32_t tiles = (smem_u32(lt_smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1), worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const uint32_t bar0 = smem_u32(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (ST + s); };
+    auto accf_bar = [&](int a) { return bar0 + 8u * (2 * ST + a); };
+    auto acce_bar = [&](int a) { return bar0 + 8u * (2 * ST + 2 + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * ST + 4);
+    volatile int *abort = &abort_flag;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < ST; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; a++) { mbar_init(accf_bar(a), 1); mbar_init(acce_bar(a), LT_EPI_WARPS * CTAS); }
+        mbar_init(drain_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<CTAS>(smem_u32(&tmem_slot), Tile::TMEM_COLS);
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    tile_sync<CTAS>();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem_base = tmem_slot;
+    const int nkb = (pr.k + LT_KB - 1) / LT_KB;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = worker; t < ntiles && ok; t += workers) {
+                const int n0 = (t % ntiles_n) * 128 * CTAS + rank * 128, m0 = (t / ntiles_n) * BN + rank * Tile::X_ROWS;
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % ST;
+                    if (!(ok = mbar_wait(empty_bar(s), ((it / ST) & 1) ^ 1, abort))) break;
+                    if (rank == 0) mbar_expect_tx(full_bar(s), (uint32_t)(CTAS * Tile::STAGE));
+                    const uint32_t dst = tiles + (uint32_t)s * Tile::STAGE;
+                    const uint32_t bar = CTAS == 1 ? full_bar(s) : rank0_address(full_bar(s));
+                    tma_load<CTAS>(dst, &map_w, bar, kb * LT_KB, n0);
+                    tma_load<CTAS>(dst + 128 * LT_KB, &map_x, bar, kb * LT_KB, m0);
+                }
+            }
+            if (!ok && rank == 0)   // the stages that were asked for last
+                for (int i = it < ST ? 0 : it - ST; i < it; i++) mbar_drain(full_bar(i % ST), (i / ST) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int t = worker; t < ntiles && ok; t += workers, n++) {
+                const int a = n & 1;
+                if (!(ok = mbar_wait(acce_bar(a), ((n >> 1) & 1) ^ 1, abort))) break;
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % ST;
+                    if (!(ok = mbar_wait(full_bar(s), (it / ST) & 1, abort))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                    const uint32_t st = tiles + (uint32_t)s * Tile::STAGE;
+                    const uint64_t adesc = umma_desc(st), bdesc = umma_desc(st + 128 * LT_KB);
+#pragma unroll
+                    for (int k = 0; k < LT_KB / 32; k++)   // 32 bytes further along k: + 2 in units of 16 bytes
+                        umma_i8<CTAS>(tmem_base + a * BN, adesc + 2 * k, bdesc + 2 * k, Tile::IDESC, (kb | k) != 0);
+                    umma_commit<CTAS>(empty_bar(s));
+                }
+                if (ok) umma_commit<CTAS>(accf_bar(a));
+            }
+            if (!ok) {   // instructions in flight read shared memory and write tensor memory
+                umma_commit<CTAS>(drain_bar);
+                mbar_drain(drain_bar, 0);
+            }
+        }
+    } else {
+        const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
+        constexpr int COLS = BN / 2;   // columns of a warp: two warps share a lane quarter
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+        int n = 0;
+        for (int t = worker; t < ntiles; t += workers, n++) {
+            const int a = n & 1;
+            const int ch = (t % ntiles_n) * 128 * CTAS + rank * 128 + quarter * 32 + lane, m0 = (t / ntiles_n) * BN + half * COLS;
+            const float ws = ch < pr.n ? pr.w_scale[ch] : 0.f, b = pr.bias && ch < pr.n ? pr.bias[ch] : 0.f;
+            if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < COLS; c += 16) {
+                int v[16];
+                tmem_ld16(lane_addr + a * BN + c, v);
+                __syncwarp();
+                if (lane < 16) scales[ew][lane] = m0 + c + lane < pr.m ? pr.x_scale[m0 + c + lane] : 0.f;
+                __syncwarp();
+                tmem_ld_wait(v);
+                T *out = (T *)pr.out + (long long)(m0 + c) * pr.out_stride + ch;
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    float y = (float)v[j] * scales[ew][j] * ws;
+                    if (pr.bias) y += b;
+                    if (ch < pr.n && m0 + c + j < pr.m) out[j * pr.out_stride] = from_float<T>(y);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader<CTAS>(acce_bar(a));
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    __syncthreads();
+    tile_sync<CTAS>();   // nobody leaves while the other CTA of the pair may still reach its barriers
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        tmem_free<CTAS>(tmem_base, Tile::TMEM_COLS);
+    }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static std::once_flag once;
+    static EncodeTiledFn fn = nullptr;
+    std::call_once(once, []() {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)p;
+    });
+    return fn;
+}
+
+int encode_rows(CUtensorMap *map, const int8_t *base, int k, int rows, long long stride, int box_rows) {
+    if (!encode_fn()) return fail(GEO_SC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {LT_KB, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? GEO_SC_OK : fail(GEO_SC_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
+}
+
+template <typename T, int CTAS, int BN> int launch_tile(const LinearParams &p, cudaStream_t s) {
+    using Tile = LinearTile<CTAS, BN>;
+    CUtensorMap map_w, map_x;
+    int rc = encode_rows(&map_w, p.w, p.k, p.n, p.w_stride, 128);
+    if (!rc) rc = encode_rows(&map_x, p.x, p.k, p.m, p.x_stride, Tile::X_ROWS);
+    if (rc) return rc;
+    static PerDeviceOnce once;
+    rc = per_device_once(once, []() -> int {
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(linear_int8_tc_kernel<T, CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::SMEM));
+        return GEO_SC_OK;
+    });
+    if (rc) return rc;
+    const int tn = (p.n + 128 * CTAS - 1) / (128 * CTAS);
+    const long long tiles = (long long)tn * ((p.m + BN - 1) / BN);
+    if (tiles > 0x3fffffff) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
+    const int workers = sm_count() / CTAS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((tiles < workers ? (int)tiles : workers) * CTAS));
+    cfg.blockDim = dim3(LT_THREADS);
+    cfg.dynamicSmemBytes = Tile::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CTAS > 1 ? 1 : 0;
+    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_int8_tc_kernel<T, CTAS, BN>, map_w, map_x, p, tn, (int)tiles));
+    return GEO_SC_OK;
+}
+
+template <typename T> int launch_tc(const LinearParams &p, cudaStream_t s) {
+    // the largest tile that still gives most SMs one
+    const long long tn = (p.n + 127) / 128, sms = sm_count();
+    if (p.m > 128 && tn * ((p.m + 255) / 256) >= sms) return launch_tile<T, 2, 256>(p, s);
+    if (p.m > 64 && tn * ((p.m + 127) / 128) >= sms) return launch_tile<T, 1, 128>(p, s);
+    return p.m <= 32 ? launch_tile<T, 1, 32>(p, s) : launch_tile<T, 1, 64>(p, s);
+}
+
+}  // namespace
+
+int launch_linear_int8_tc(const LinearParams &p, int dtype, cudaStream_t s) {
+    if (dtype == GEO_SC_DTYPE_F32) return launch_tc<float>(p, s);
+    if (dtype == GEO_SC_DTYPE_BF16) return launch_tc<__nv_bfloat16>(p, s);
+    return launch_tc<__half>(p, s);
+}
+
+int linear_int8_tc_error_count(int *count) {
+    GEO_CUDA_CHECK(cudaMemcpyFromSymbol(count, g_linear_tc_errors, sizeof(int)));
+    return GEO_SC_OK;
+}
+
+}  // namespace geo
