@@ -9,11 +9,17 @@
 // q * scale is the normalised row.  The norm's factor cancels out of q, so the integers depend on the row's values
 // alone and not on the order in which the squares are added: a row gives the same integers on every launch shape.  A
 // thread computes 127 p / max|p| in 32 bits and decides it in 64 only where the 32-bit value lies within 2^-14 of a
-// border between two integers (its error is below 127 * 2^-23 = 2^-16): one value in about eight thousand.
+// border between two integers (its error is below 2^-16): one value in about eight thousand.
 //
-// What bounds it: HBM.  One read of x and residual, one write of r, q and the scales; a row stays in registers between
-// the statistics and the rounding.  Squares are summed in 32 bits per thread and joined in 64; a row whose sum leaves
-// the range of 32 bits (values above 1e19, or so small that their squares vanish) is summed again in 64.
+// What bounds it: HBM.  One read of x and residual, one write of r, q and the scales.  CTAs walk over rows; while a row is
+// reduced and rounded, the next two are on their way into shared memory (cp.async, three stages), so that the copies do
+// not stop for the barriers of the reduction.  Squares are summed in 32 bits per thread; a row whose sum leaves their
+// range (values above 1e18, or so small that their squares vanish) is read and summed again in 64.
+//
+// norm_int8_kernel: rows that start on 16-byte boundaries and are whole numbers of 16-byte vectors.  A thread copies the
+// vectors that it computes itself, so the stages need no barrier; the products stay in registers from the statistics to
+// the rounding.  norm_int8_ragged_kernel: every other row.  Its 16-byte granules are copied as they lie in memory, and the
+// threads read them value by value, neighbours next to each other.
 #include "sc_rows8.h"
 
 namespace geo {
@@ -25,193 +31,440 @@ struct NormParams {
     int8_t *q;
     float *scale;
     long long rows, x_stride, res_stride, q_stride;
-    int cols, weight_dtype;
+    int cols;
     float eps;
 };
 
-__device__ __forceinline__ float weight_at(const NormParams &p, int c) {
-    if (p.weight_dtype == GEO_SC_DTYPE_F32) return __ldg((const float *)p.weight + c);
-    if (p.weight_dtype == GEO_SC_DTYPE_BF16) return __bfloat162float(__ldg((const __nv_bfloat16 *)p.weight + c));
-    return __half2float(__ldg((const __half *)p.weight + c));
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN is kept
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-// 127 p / top as the nearest integer, half to even (see above); |p| <= top, top > 0 and finite.
-__device__ __forceinline__ int round_to_top(float p, float top, float inv) {
-    const float t = p * inv;
-    const float off = fabsf(t - rintf(t));
-    if (off > 0.5f - 6.2e-5f || top < 1e-30f)   // next to a border, or a reciprocal outside the normal range
-        return (int)rint((double)p * 127.0 / (double)top);
-    return __float2int_rn(t);
-}
-
-template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> row_values(const T *x, const T *res, long long at) {
-    Pack<T, VEC> v = load_pack<T, VEC>(x + at);
-    if (res) {
-        const Pack<T, VEC> u = load_pack<T, VEC>(res + at);
+// VEC products as integers: 127 p / top, half to even; |p| <= top, 1e-30 <= top, finite; inv = 127 / top in fp32.
+// p * inv + 1.5 * 2^23 rounds to an integer whose two's complement is the sum's low byte.  Next to a border h between
+// two integers the sign of 127 p - h top decides, whose products are exact in 64 bits.
+template <int VEC> __device__ __forceinline__ Pack<int8_t, VEC> round_pack(const float (&p)[VEC], float top, float inv) {
+    constexpr float MAGIC = 12582912.f, NEAR = 0.5f - 6.2e-5f;
+    float off = 0.f;
+    uint32_t m[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) v.v[e] = from_float<T>(to_float(v.v[e]) + to_float(u.v[e]));
+    for (int e = 0; e < VEC; e++) {
+        const float t = fmaf(p[e], inv, MAGIC);
+        off = fmaxf(off, fabsf(fmaf(p[e], inv, MAGIC - t)));
+        m[e] = __float_as_uint(t);
+    }
+    if (off > NEAR) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float r = __uint_as_float(m[e]) - MAGIC, f = fmaf(p[e], inv, -r);
+            if (fabsf(f) > NEAR) {
+                const float h = r + copysignf(0.5f, f);
+                const double side = fma(127.0, (double)p[e], -(double)h * (double)top);
+                m[e] = __float_as_uint(MAGIC + (side > 0 ? h + 0.5f : side < 0 ? h - 0.5f : rintf(h)));
+            }
+        }
+    }
+    Pack<int8_t, VEC> o;
+    if constexpr (VEC == 1) {
+        o.v[0] = (int8_t)m[0];
+    } else {
+        uint32_t *word = reinterpret_cast<uint32_t *>(&o);
+#pragma unroll
+        for (int i = 0; i < VEC / 4; i++)
+            word[i] = __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
+    }
+    return o;
+}
+
+template <typename T, int VEC> __device__ __forceinline__ void add_pack(Pack<T, VEC> &v, const Pack<T, VEC> &u) {
+    float a[VEC], b[VEC];
+    unpack<VEC>(v, a);
+    unpack<VEC>(u, b);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) a[e] += b[e];
+    pack<VEC>(v, a);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {   // 16 bytes, zeros past `bytes`
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// Statistics of a row, joined over its tpr threads (one or more warps of a CTA; part_* have room for two turns).
+struct RowStats {
+    float ss, top;
+    bool again;   // the sum of squares has to be taken again in 64 bits; the same for the whole CTA
+};
+template <bool NORM>
+__device__ __forceinline__ RowStats join_stats(float ss, float top, int tpr, int first, float (*part_ss)[32], float (*part_top)[32], int turn) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = tpr >> 5;
+    if (NORM) ss = warp_sum(ss);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    RowStats r;
+    // infinite (or NaN) without a product that is, or vanished without being zero
+    r.again = NORM && top <= 3.402823466e38f && (!(ss <= 3.0e37f) || (ss < 1e-30f && top > 0.f));
+    if (tpr > 32) {
+        if (lane == 0) {
+            part_ss[turn][warp] = ss;
+            part_top[turn][warp] = top;
+        }
+        r.again = __syncthreads_or(r.again);
+        // one partial per lane, joined in the same order by every warp
+        top = part_top[turn][first + (lane & (wpr - 1))];
+        ss = NORM ? part_ss[turn][first + (lane & (wpr - 1))] : 0.f;
+        for (int o = 1; o < wpr; o *= 2) {
+            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+    }
+    r.ss = ss;
+    r.top = top;
+    return r;
+}
+
+// The scale of a row from its statistics; total: the sum of squares in 64 bits where it was taken again.
+template <bool NORM> __device__ __forceinline__ float row_scale(const RowStats &st, double total, int cols, float eps) {
+    if (!(st.top <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
+    if (!NORM || st.top == 0.f) return st.top / 127.f;
+    if (st.again) return (float)((double)st.top / 127.0 / sqrt(total / cols + (double)eps));
+    return st.top / sqrtf(st.ss / (float)cols + eps) / 127.f;
+}
+
+// Joins the 64-bit sums of a row (every thread of the CTA takes part).
+__device__ __forceinline__ double join_sum64(double v, int tpr, int first, double *part) {
+    v = warp_sum(v);
+    if (tpr > 32) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0;
+        for (int i = 0; i < tpr >> 5; i++) v += part[first + i];
+        __syncthreads();
     }
     return v;
 }
 
-// TPR threads own a row, VEC values per load, NV loads kept in registers (longer rows read the rest a second time).
-template <typename T, int VEC, int NV, bool NORM>
+// tpr threads own a row, VEC values per 16-byte vector, NV vectors of a thread in the stages (longer rows read the rest
+// from memory, twice).  W: the weight's type; without NORM there is none.
+template <typename T, typename W, int NV, bool NORM>
 __global__ void __launch_bounds__(1024) norm_int8_kernel(NormParams pr, int tpr) {
-    __shared__ float part_ss[32];
-    __shared__ unsigned part_top[32];
-    __shared__ double part_ss64[32];
-    const int tid = threadIdx.x % tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
-    const bool live = row < pr.rows;
-    const int nvec = live ? pr.cols / VEC : 0;
-    const T *x = (const T *)pr.x + (live ? row * pr.x_stride : 0);
-    const T *res = pr.residual ? (const T *)pr.residual + (live ? row * pr.res_stride : 0) : nullptr;
-    T *sum_out = pr.sum_out ? (T *)pr.sum_out + (live ? row * (long long)pr.cols : 0) : nullptr;
+    constexpr int VEC = 16 / sizeof(T), STAGES = 3;
+    extern __shared__ __align__(16) unsigned char norm_smem[];
+    __shared__ float part_ss[2][32], part_top[2][32];
+    __shared__ double part64[32];
+    const int tid = threadIdx.x % tpr, rpc = blockDim.x / tpr, group = threadIdx.x / tpr, first = group * (tpr >> 5);
+    const int nvec = pr.cols / VEC;
+    const bool has_res = pr.residual != nullptr;
+    const T *const x = (const T *)pr.x, *const res = (const T *)pr.residual;
+    T *const sum_out = (T *)pr.sum_out;
+    const long long step = (long long)gridDim.x * rpc;
+    // a thread's vectors: [stage][x, residual][NV], blockDim.x vectors apart
+    const uint32_t slot_bytes = blockDim.x * 16, stage_bytes = slot_bytes * NV * (has_res ? 2 : 1);
+    unsigned char *const mine_at = norm_smem + threadIdx.x * 16;
 
-    Pack<T, VEC> keep[NV];
-    float ss = 0.f;
-    unsigned top = 0;   // |p| as its bit pattern: ordered like the values, NaN above infinity, so that neither is lost
-    auto take = [&](const Pack<T, VEC> &v, int i) {
+    auto weight_of = [&](int i, float (&w)[VEC]) {
+        if constexpr (NORM) {
+            if constexpr (VEC * sizeof(W) == 32) {   // fp32 weights of 16-bit values: two loads
+                const Pack<W, VEC / 2> a = load_pack<W, VEC / 2>((const W *)pr.weight + i * VEC), b = load_pack<W, VEC / 2>((const W *)pr.weight + i * VEC + VEC / 2);
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const float r = to_float(v.v[e]);
-            if (NORM) ss = fmaf(r, r, ss);
-            const float p = pr.weight ? r * weight_at(pr, i * VEC + e) : r;
-            top = max(top, __float_as_uint(p) & 0x7fffffffu);
+                for (int e = 0; e < VEC / 2; e++) {
+                    w[e] = to_float(a.v[e]);
+                    w[VEC / 2 + e] = to_float(b.v[e]);
+                }
+            } else {
+                unpack<VEC>(load_pack<W, VEC>((const W *)pr.weight + i * VEC), w);
+            }
         }
     };
+    auto ask = [&](long long row, int stage) {
+        if (row < pr.rows) {
+            const T *px = x + row * pr.x_stride, *pq = res + row * pr.res_stride;
+            const uint32_t dst = smem_u32(mine_at) + stage * stage_bytes;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-        if (tid + j * tpr < nvec) keep[j] = row_values<T, VEC>(x, res, (long long)(tid + j * tpr) * VEC);
+            for (int j = 0; j < NV; j++)
+                if (tid + j * tpr < nvec) {
+                    copy_async(dst + j * slot_bytes, px + (tid + j * tpr) * VEC, 16);
+                    if (has_res) copy_async(dst + (NV + j) * slot_bytes, pq + (tid + j * tpr) * VEC, 16);
+                }
+        }
+        copy_commit();
+    };
+    const long long start = (long long)blockIdx.x * rpc;
+    ask(start + group, 0);
+    ask(start + step + group, 1);
+    int turn = 0, stage = 0;
+    // every thread of a CTA makes the same number of turns; rows past the end take part in the barriers only
+    for (long long base = start; base < pr.rows; base += step, turn ^= 1) {
+        const long long row = base + group;
+        const int mine = row < pr.rows ? nvec : 0;
+        ask(row + 2 * step, stage == 0 ? 2 : stage - 1);
+        copy_wait<2>();
+        float p[NV][VEC], ss = 0.f, top = 0.f;
+        auto take = [&](const Pack<T, VEC> &v, int i, float (&pv)[VEC]) {
+            float r[VEC], wv[VEC];
+            unpack<VEC>(v, r);
+            weight_of(i, wv);
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-        if (tid + j * tpr < nvec) {
-            if (sum_out) store_pack<T, VEC>(sum_out + (long long)(tid + j * tpr) * VEC, keep[j]);
-            take(keep[j], tid + j * tpr);
-        }
-    for (int i = tid + NV * tpr; i < nvec; i += tpr) {
-        const Pack<T, VEC> v = row_values<T, VEC>(x, res, (long long)i * VEC);
-        if (sum_out) store_pack<T, VEC>(sum_out + (long long)i * VEC, v);
-        take(v, i);
-    }
-
-    ss = warp_sum(ss);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) {
-        part_ss[warp] = ss;
-        part_top[warp] = top;
-    }
-    __syncthreads();
-    // every warp of the CTA looks at every partial, so that all of them agree on whether any row is summed again
-    const int warps = blockDim.x >> 5, wpr = tpr >> 5, first = (threadIdx.x / tpr) * wpr;
-    double total = 0;
-    bool again = false;
-    top = 0;
-    for (int w = 0; w < warps; w++) {
-        const float s = part_ss[w];
-        const unsigned t = part_top[w];
-        if (NORM && t < 0x7f800000u && (!(s <= 3.0e38f) || (s < 1e-30f && t > 0))) again = true;
-        if (w >= first && w < first + wpr) {
-            total += (double)s;
-            top = max(top, t);
-        }
-    }
-    if (NORM && again) {
-        double s64 = 0;
+            for (int e = 0; e < VEC; e++) {
+                if (NORM) ss = fmaf(r[e], r[e], ss);
+                pv[e] = NORM ? r[e] * wv[e] : r[e];
+                top = max_nan(top, fabsf(pv[e]));
+            }
+        };
+        // a vector from memory: past the stages' part of the row, or once more
+        auto far = [&](int i, bool write) {
+            Pack<T, VEC> v = load_pack<T, VEC>(x + row * pr.x_stride + (long long)i * VEC);
+            if (has_res) {
+                add_pack<T, VEC>(v, load_pack<T, VEC>(res + row * pr.res_stride + (long long)i * VEC));
+                if (write) store_pack<T, VEC>(sum_out + row * pr.cols + (long long)i * VEC, v);
+            }
+            return v;
+        };
+        const unsigned char *const at = mine_at + stage * stage_bytes;
 #pragma unroll
         for (int j = 0; j < NV; j++)
-            if (tid + j * tpr < nvec)
-                for (int e = 0; e < VEC; e++) s64 += (double)to_float(keep[j].v[e]) * (double)to_float(keep[j].v[e]);
-        for (int i = tid + NV * tpr; i < nvec; i += tpr) {
-            const Pack<T, VEC> v = row_values<T, VEC>(x, res, (long long)i * VEC);
-            for (int e = 0; e < VEC; e++) s64 += (double)to_float(v.v[e]) * (double)to_float(v.v[e]);
+            if (tid + j * tpr < mine) {
+                Pack<T, VEC> v = *(const Pack<T, VEC> *)(at + j * slot_bytes);
+                if (has_res) {
+                    add_pack<T, VEC>(v, *(const Pack<T, VEC> *)(at + (NV + j) * slot_bytes));
+                    store_pack<T, VEC>(sum_out + row * pr.cols + (tid + j * tpr) * VEC, v);
+                }
+                take(v, tid + j * tpr, p[j]);
+            }
+        for (int i = tid + NV * tpr; i < mine; i += tpr) {
+            float pv[VEC];
+            take(far(i, true), i, pv);
         }
-        s64 = warp_sum(s64);
-        if (lane == 0) part_ss64[warp] = s64;
-        __syncthreads();
-        total = 0;
-        for (int w = first; w < first + wpr; w++) total += part_ss64[w];
-    }
-    if (!live) return;
-    const float ftop = __uint_as_float(top);
-    double scale = (double)ftop / 127.0;
-    if (NORM && top > 0) scale /= sqrt(total / pr.cols + (double)pr.eps);
-    const bool fine = top < 0x7f800000u && (float)scale <= 3.402823466e38f;
-    if (tid == 0) pr.scale[row] = fine ? (float)scale : __int_as_float(0x7fc00000);
+        stage = stage == 2 ? 0 : stage + 1;
 
-    const float inv = 127.f / ftop;
-    const bool zero = !fine || top == 0;
-    int8_t *q = pr.q + row * pr.q_stride;
-    auto give = [&](const Pack<T, VEC> &v, int i) {
-        Pack<int8_t, VEC> o;
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const float r = to_float(v.v[e]);
-            const float p = pr.weight ? r * weight_at(pr, i * VEC + e) : r;
-            o.v[e] = zero ? 0 : (int8_t)round_to_top(p, ftop, inv);
+        const RowStats st = join_stats<NORM>(ss, top, tpr, first, part_ss, part_top, turn);
+        double total = 0;
+        if (NORM && st.again) {
+            for (int i = tid; i < mine; i += tpr) {
+                float r[VEC];
+                unpack<VEC>(far(i, false), r);
+                for (int e = 0; e < VEC; e++) total += (double)r[e] * (double)r[e];
+            }
+            total = join_sum64(total, tpr, first, part64);
         }
-        store_pack<int8_t, VEC>(q + (long long)i * VEC, o);
-    };
+        if (mine == 0) continue;
+        if (tid == 0) pr.scale[row] = row_scale<NORM>(st, total, pr.cols, pr.eps);
+
+        const bool zero = !(st.top <= 3.402823466e38f) || st.top == 0.f;
+        // products below the normal range of a reciprocal: the integers are those of 2^64 times the row
+        const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = 127.f / lifted;
+        int8_t *q = pr.q + row * pr.q_stride;
+        auto give = [&](float (&pv)[VEC], int i) {
+            Pack<int8_t, VEC> o = {};
+            if (lift != 1.f)
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-        if (tid + j * tpr < nvec) give(keep[j], tid + j * tpr);
-    for (int i = tid + NV * tpr; i < nvec; i += tpr) give(row_values<T, VEC>(x, res, (long long)i * VEC), i);
+                for (int e = 0; e < VEC; e++) pv[e] *= lift;
+            if (!zero) o = round_pack<VEC>(pv, lifted, inv);
+            store_pack<int8_t, VEC>(q + (long long)i * VEC, o);
+        };
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (tid + j * tpr < mine) give(p[j], tid + j * tpr);
+        for (int i = tid + NV * tpr; i < mine; i += tpr) {
+            float pv[VEC];
+            take(far(i, false), i, pv);
+            give(pv, i);
+        }
+    }
+    copy_wait<0>();
 }
 
-template <typename T, int VEC, int NV> int launch_norm_v(const NormParams &p, bool norm, cudaStream_t s) {
-    const long long nvec = p.cols / VEC;
-    // few rows: every load of a row in flight at once; many rows: NV loads per thread, more rows per SM
-    const long long want = p.rows < 2LL * sm_count() ? nvec : (nvec + NV - 1) / NV;
-    int tpr = 32;
-    while (tpr < 1024 && tpr < want) tpr *= 2;
-    const int threads = tpr < 128 && p.rows > 1 ? 128 : tpr;
-    const long long grid = (p.rows + threads / tpr - 1) / (threads / tpr);
-    if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows", p.rows);
-    if (norm) norm_int8_kernel<T, VEC, NV, true><<<(unsigned)grid, threads, 0, s>>>(p, tpr);
-    else norm_int8_kernel<T, VEC, NV, false><<<(unsigned)grid, threads, 0, s>>>(p, tpr);
+// One row per CTA at a time, any alignment.  stages: 3, or 1 where three rows do not fit, or 0 (read from memory).
+template <typename T, typename W, bool NORM>
+__global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, int stages, int buf_bytes) {
+    extern __shared__ __align__(16) unsigned char norm_smem[];
+    __shared__ float part_ss[2][32], part_top[2][32];
+    __shared__ double part64[32];
+    const int tid = threadIdx.x, threads = blockDim.x, cols = pr.cols;
+    const bool has_res = pr.residual != nullptr;
+    const T *const x = (const T *)pr.x, *const res = (const T *)pr.residual;
+    T *const sum_out = (T *)pr.sum_out;
+    const int stage_bytes = buf_bytes * (has_res ? 2 : 1);
+
+    // The 16-byte granules of a row, each at its own distance from the one with the row's first byte.  A granule is read
+    // from the row's first byte on (value by value) where it begins before it, and up to the row's last byte.
+    auto copy_row = [&](const T *row, unsigned char *buf) {
+        const uintptr_t a = (uintptr_t)row, e = a + (size_t)cols * sizeof(T), g0 = a & ~(uintptr_t)15;
+        const int granules = (int)((e - g0 + 15) >> 4);
+        for (int i = tid; i < granules; i += threads) {
+            const uintptr_t g = g0 + (uintptr_t)i * 16;
+            if (g < a) {
+                const int n = (int)(min(e, g + 16) - a) / (int)sizeof(T);
+                for (int k = 0; k < n; k++) *(T *)(buf + (a - g0) + k * sizeof(T)) = row[k];
+            } else {
+                copy_async(smem_u32(buf) + i * 16, (const void *)g, (int)(min(e, g + 16) - g));
+            }
+        }
+    };
+    auto ask = [&](long long row, int stage) {
+        if (row < pr.rows) {
+            copy_row(x + row * pr.x_stride, norm_smem + stage * stage_bytes);
+            if (has_res) copy_row(res + row * pr.res_stride, norm_smem + stage * stage_bytes + buf_bytes);
+        }
+        copy_commit();
+    };
+    if (stages == 3) {
+        ask(blockIdx.x, 0);
+        ask((long long)blockIdx.x + gridDim.x, 1);
+    }
+    int turn = 0, stage = 0;
+    for (long long row = blockIdx.x; row < pr.rows; row += gridDim.x, turn ^= 1) {
+        const T *px = x + row * pr.x_stride, *pq = has_res ? res + row * pr.res_stride : nullptr;
+        if (stages == 3) {
+            ask(row + 2LL * gridDim.x, stage == 0 ? 2 : stage - 1);
+            copy_wait<2>();
+        } else if (stages == 1) {
+            ask(row, 0);
+            copy_wait<0>();
+        }
+        if (stages) {
+            __syncthreads();
+            px = (const T *)(norm_smem + stage * stage_bytes + ((uintptr_t)px & 15));
+            if (has_res) pq = (const T *)(norm_smem + stage * stage_bytes + buf_bytes + ((uintptr_t)pq & 15));
+        }
+        auto value = [&](int c) {
+            float r = to_float(px[c]);
+            if (has_res) r = to_float(from_float<T>(r + to_float(pq[c])));
+            return r;
+        };
+        auto product = [&](float r, int c) {
+            if constexpr (NORM) return r * to_float(((const W *)pr.weight)[c]);
+            else return r;
+        };
+        float ss = 0.f, top = 0.f;
+#pragma unroll 4
+        for (int c = tid; c < cols; c += threads) {
+            const float r = value(c);
+            if (has_res) sum_out[row * cols + c] = from_float<T>(r);
+            if (NORM) ss = fmaf(r, r, ss);
+            top = max_nan(top, fabsf(product(r, c)));
+        }
+        const RowStats st = join_stats<NORM>(ss, top, threads, 0, part_ss, part_top, turn);
+        double total = 0;
+        if (NORM && st.again) {
+            for (int c = tid; c < cols; c += threads) total += (double)value(c) * (double)value(c);
+            total = join_sum64(total, threads, 0, part64);
+        }
+        if (tid == 0) pr.scale[row] = row_scale<NORM>(st, total, cols, pr.eps);
+        const bool zero = !(st.top <= 3.402823466e38f) || st.top == 0.f;
+        const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = 127.f / lifted;
+        int8_t *q = pr.q + row * pr.q_stride;
+#pragma unroll 4
+        for (int c = tid; c < cols; c += threads) {
+            const float p[1] = {product(value(c), c) * lift};
+            q[c] = zero ? 0 : round_pack<1>(p, lifted, inv).v[0];
+        }
+        if (stages) __syncthreads();   // the stage may be overwritten
+        if (stages == 3) stage = stage == 2 ? 0 : stage + 1;
+    }
+    copy_wait<0>();
+}
+
+constexpr int NORM_SMEM = 200 * 1024;   // of an SM's 227 KB, shared by its CTAs
+
+template <typename T, typename W, int NV, bool NORM> int launch_norm_nv(const NormParams &p, int tpr, cudaStream_t s) {
+    const int threads = tpr < 256 && p.rows > 1 ? 256 : tpr, rpc = threads / tpr;
+    const int smem = threads * 16 * NV * (p.residual ? 2 : 1) * 3;
+    static PerDeviceOnce once;
+    int rc = per_device_once(once, []() -> int {
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_kernel<T, W, NV, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
+        return GEO_SC_OK;
+    });
+    if (rc) return rc;
+    // as many CTAs as fit 1024 threads of 64 registers and the stages on every SM
+    const long long need = (p.rows + rpc - 1) / rpc, most = (long long)sm_count() * max(1, min(1024 / threads, NORM_SMEM / smem));
+    norm_int8_kernel<T, W, NV, NORM><<<(unsigned)(need < most ? need : most), threads, smem, s>>>(p, tpr);
     GEO_CUDA_CHECK(cudaGetLastError());
     return GEO_SC_OK;
 }
 
-template <typename T> int launch_norm(const NormParams &p, bool norm, cudaStream_t s) {
+template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p, cudaStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
-    // whole 16-byte loads where every row starts on a 16-byte boundary and ends on one; else value by value
+    // whole 16-byte vectors where every row starts on a 16-byte boundary and ends on one
     const bool wide = p.cols % VEC == 0 && aligned_to(p.x, 16) && p.x_stride % VEC == 0 && (!p.residual || (aligned_to(p.residual, 16) && p.res_stride % VEC == 0)) &&
-                      (!p.sum_out || aligned_to(p.sum_out, 16)) && aligned_to(p.q, VEC) && p.q_stride % VEC == 0;
-    return wide ? launch_norm_v<T, VEC, 4>(p, norm, s) : launch_norm_v<T, 1, 16>(p, norm, s);
+                      (!p.sum_out || aligned_to(p.sum_out, 16)) && aligned_to(p.q, VEC) && p.q_stride % VEC == 0 && (!NORM || aligned_to(p.weight, 16));
+    if (wide) {
+        // few rows: one vector per thread, the shortest way through a row; many: two, for half the reductions
+        const int nvec = p.cols / VEC, want = p.rows < 2LL * sm_count() ? nvec : (nvec + 1) / 2;
+        int tpr = 32;
+        while (tpr < 1024 && tpr < want) tpr *= 2;
+        return nvec <= tpr ? launch_norm_nv<T, W, 1, NORM>(p, tpr, s) : launch_norm_nv<T, W, 2, NORM>(p, tpr, s);
+    }
+    int threads = 64;
+    while (threads < 1024 && threads * 8 < p.cols) threads *= 2;
+    const long long buf = ((long long)p.cols * sizeof(T) + 47) / 16 * 16, stage = buf * (p.residual ? 2 : 1);
+    const int stages = stage * 3 <= NORM_SMEM / 2 ? 3 : stage <= NORM_SMEM ? 1 : 0, smem = (int)(stages * stage);
+    static PerDeviceOnce once;
+    int rc = per_device_once(once, []() -> int {
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_ragged_kernel<T, W, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
+        return GEO_SC_OK;
+    });
+    if (rc) return rc;
+    const long long most = (long long)sm_count() * max(1, min(1024 / threads, smem ? NORM_SMEM / smem : 16));
+    norm_int8_ragged_kernel<T, W, NORM><<<(unsigned)(p.rows < most ? p.rows : most), threads, smem, s>>>(p, stages, (int)buf);
+    GEO_CUDA_CHECK(cudaGetLastError());
+    return GEO_SC_OK;
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t *q, long long q_stride, const float *scale, T *out, long long rows, int cols) {
-    const int nvec = cols / VEC;
-    const long long n = rows * nvec;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long row = n <= 0xffffffffLL ? (long long)((unsigned)i / (unsigned)nvec) : i / nvec;
-        const int c = (int)(i - row * nvec) * VEC;
-        const Pack<int8_t, VEC> v = load_pack<int8_t, VEC>(q + row * q_stride + c);
-        const float s = __ldg(scale + row);
-        Pack<T, VEC> o;
+// A warp takes STEPS x 32 vectors of a row (read VEC integers, write VEC values), all steps in flight at once.
+template <typename T, int VEC, int STEPS>
+__global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t *q, long long q_stride, const float *scale, T *out, long long units, int upr,
+                                                               int nvec, int cols) {
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= units) return;
+    const long long row = units <= 0xffffffffLL ? (long long)((unsigned)unit / (unsigned)upr) : unit / upr;
+    const int first = (int)(unit - row * upr) * (32 * STEPS) + (threadIdx.x & 31);
+    q += row * q_stride;
+    out += row * cols;
+    Pack<int8_t, VEC> v[STEPS];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) o.v[e] = from_float<T>((float)v.v[e] * s);
-        store_pack<T, VEC>(out + row * cols + c, o);
-    }
+    for (int j = 0; j < STEPS; j++)
+        if (first + j * 32 < nvec) v[j] = load_pack<int8_t, VEC>(q + (long long)(first + j * 32) * VEC);
+    const float s = __ldg(scale + row);
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+        if (first + j * 32 < nvec) {
+            Pack<T, VEC> o;
+            float f[VEC];
+            if constexpr (VEC == 1) {
+                f[0] = (float)v[j].v[0] * s;
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) unpack_bytes(reinterpret_cast<const uint32_t *>(&v[j])[e / 4], f + e);
+#pragma unroll
+                for (int e = 0; e < VEC; e++) f[e] *= s;
+            }
+            pack<VEC>(o, f);
+            store_pack<T, VEC>(out + (long long)(first + j * 32) * VEC, o);
+        }
+}
+
+template <typename T, int VEC, int STEPS> int launch_dequantize_v(long long rows, int cols, const int8_t *q, long long q_stride, const float *scale, T *out, cudaStream_t s) {
+    const int nvec = cols / VEC, upr = (nvec + 32 * STEPS - 1) / (32 * STEPS);
+    const long long units = rows * upr, grid = (units + 7) / 8;
+    if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows of %d values", rows, cols);
+    dequantize_int8_kernel<T, VEC, STEPS><<<(unsigned)grid, 256, 0, s>>>(q, q_stride, scale, out, units, upr, nvec, cols);
+    GEO_CUDA_CHECK(cudaGetLastError());
+    return GEO_SC_OK;
 }
 
 template <typename T> int launch_dequantize(long long rows, int cols, const int8_t *q, long long q_stride, const float *scale, T *out, cudaStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
     const bool wide = cols % VEC == 0 && aligned_to(q, VEC) && q_stride % VEC == 0 && aligned_to(out, 16);
-    const long long n = rows * (wide ? cols / VEC : cols);
-    const long long want = (n + 255) / 256, most = 16LL * sm_count();
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    if (wide) dequantize_int8_kernel<T, VEC><<<grid, 256, 0, s>>>(q, q_stride, scale, out, rows, cols);
-    else dequantize_int8_kernel<T, 1><<<grid, 256, 0, s>>>(q, q_stride, scale, out, rows, cols);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    return wide ? launch_dequantize_v<T, VEC, 4>(rows, cols, q, q_stride, scale, out, s) : launch_dequantize_v<T, 1, 16>(rows, cols, q, q_stride, scale, out, s);
 }
 
 int check_rows(long long rows, int cols, int dtype) {
     if (rows < 0 || cols < 1) return fail(GEO_SC_ERR_SHAPE, "%lld rows of %d values", rows, cols);
-    if (rows > (1LL << 40) / cols) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows of %d values", rows, cols);
+    if (cols > (1 << 30) || rows > (1LL << 40) / cols) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows of %d values", rows, cols);
     if (!dtype_known(dtype)) return fail(GEO_SC_ERR_UNSUPPORTED, "unknown element type %d", dtype);
     return GEO_SC_OK;
 }
@@ -231,14 +484,16 @@ int geo_sc_rms_norm_int8(long long rows, int cols, int dtype, const void *x, lon
     if (rows == 0) return GEO_SC_OK;
     if (!x || !weight || !q || !scale) return fail(GEO_SC_ERR_NULL, "x, weight, q and scale are required");
     if ((residual == nullptr) != (sum_out == nullptr)) return fail(GEO_SC_ERR_NULL, "residual and sum_out come together");
-    if (!dtype_known(weight_dtype)) return fail(GEO_SC_ERR_UNSUPPORTED, "unknown weight type %d", weight_dtype);
+    if (weight_dtype != GEO_SC_DTYPE_F32 && weight_dtype != dtype)
+        return fail(GEO_SC_ERR_UNSUPPORTED, "weight has to be fp32 or of the type of x, not type %d", weight_dtype);
     if (!(eps >= 0.f) || eps > 3.402823466e38f) return fail(GEO_SC_ERR_SHAPE, "eps must be finite and not negative");
     if (x_stride < 0 || residual_stride < 0 || q_stride < cols) return fail(GEO_SC_ERR_SHAPE, "bad row stride");
-    NormParams p{x, residual, weight, sum_out, q, scale, rows, x_stride, residual_stride, q_stride, cols, weight_dtype, eps};
+    NormParams p{x, residual, weight, sum_out, q, scale, rows, x_stride, residual_stride, q_stride, cols, eps};
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == GEO_SC_DTYPE_F32) return launch_norm<float>(p, true, s);
-    if (dtype == GEO_SC_DTYPE_BF16) return launch_norm<__nv_bfloat16>(p, true, s);
-    return launch_norm<__half>(p, true, s);
+    const bool f32 = weight_dtype == GEO_SC_DTYPE_F32;
+    if (dtype == GEO_SC_DTYPE_F32) return launch_norm<float, float, true>(p, s);
+    if (dtype == GEO_SC_DTYPE_BF16) return f32 ? launch_norm<__nv_bfloat16, float, true>(p, s) : launch_norm<__nv_bfloat16, __nv_bfloat16, true>(p, s);
+    return f32 ? launch_norm<__half, float, true>(p, s) : launch_norm<__half, __half, true>(p, s);
 }
 
 int geo_sc_quantize_int8(long long rows, int cols, int dtype, const void *x, long long x_stride, int8_t *q, long long q_stride,
@@ -248,11 +503,11 @@ int geo_sc_quantize_int8(long long rows, int cols, int dtype, const void *x, lon
     if (rows == 0) return GEO_SC_OK;
     if (!x || !q || !scale) return fail(GEO_SC_ERR_NULL, "x, q and scale are required");
     if (x_stride < 0 || q_stride < cols) return fail(GEO_SC_ERR_SHAPE, "bad row stride");
-    NormParams p{x, nullptr, nullptr, nullptr, q, scale, rows, x_stride, 0, q_stride, cols, GEO_SC_DTYPE_F32, 0.f};
+    NormParams p{x, nullptr, nullptr, nullptr, q, scale, rows, x_stride, 0, q_stride, cols, 0.f};
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == GEO_SC_DTYPE_F32) return launch_norm<float>(p, false, s);
-    if (dtype == GEO_SC_DTYPE_BF16) return launch_norm<__nv_bfloat16>(p, false, s);
-    return launch_norm<__half>(p, false, s);
+    if (dtype == GEO_SC_DTYPE_F32) return launch_norm<float, float, false>(p, s);
+    if (dtype == GEO_SC_DTYPE_BF16) return launch_norm<__nv_bfloat16, __nv_bfloat16, false>(p, s);
+    return launch_norm<__half, __half, false>(p, s);
 }
 
 int geo_sc_dequantize_int8(long long rows, int cols, const int8_t *q, long long q_stride, const float *scale, int dtype, void *out,

@@ -26,6 +26,65 @@ template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, co
     *reinterpret_cast<Pack<T, N> *>(p) = v;
 }
 
+// Packs to and from fp32, two 16-bit values per instruction.
+template <int N> __device__ __forceinline__ void unpack(const Pack<float, N> &v, float (&f)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] = v.v[e];
+}
+template <int N> __device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, N> &v, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = __bfloat162float(v.v[0]);
+    } else {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) {
+            f[2 * e] = __uint_as_float(w[e] << 16);
+            f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void unpack(const Pack<__half, N> &v, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = __half2float(v.v[0]);
+    } else {
+        const __half2 *w = reinterpret_cast<const __half2 *>(&v);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) {
+            const float2 t = __half22float2(w[e]);
+            f[2 * e] = t.x;
+            f[2 * e + 1] = t.y;
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void pack(Pack<float, N> &v, const float (&f)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; e++) v.v[e] = f[e];
+}
+template <int N> __device__ __forceinline__ void pack(Pack<__nv_bfloat16, N> &v, const float (&f)[N]) {
+    if constexpr (N == 1) {
+        v.v[0] = __float2bfloat16_rn(f[0]);
+    } else {
+        __nv_bfloat162 *w = reinterpret_cast<__nv_bfloat162 *>(&v);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) w[e] = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+    }
+}
+template <int N> __device__ __forceinline__ void pack(Pack<__half, N> &v, const float (&f)[N]) {
+    if constexpr (N == 1) {
+        v.v[0] = __float2half_rn(f[0]);
+    } else {
+        __half2 *w = reinterpret_cast<__half2 *>(&v);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) w[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+    }
+}
+// Four signed bytes as floats: a byte b + 128 in the low mantissa of 2^23 is the float 2^23 + 128 + b, exactly.
+__device__ __forceinline__ void unpack_bytes(uint32_t w, float *f) {
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int e = 0; e < 4; e++) f[e] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + e)) - 8388736.f;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

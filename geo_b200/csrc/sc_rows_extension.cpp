@@ -98,7 +98,8 @@ at::TensorOptions floats(const Tensor &like) { return like.options().dtype(at::k
 
 py::tuple rms_norm_int8(const Tensor &x, const Tensor &weight, const OptTensor &residual_, double eps) {
     const Tensor *residual = ptr(residual_);
-    const int code = dtype_code(x.scalar_type(), "x"), wcode = dtype_code(weight.scalar_type(), "weight");
+    const int code = dtype_code(x.scalar_type(), "x");
+    dtype_code(weight.scalar_type(), "weight");
     check_rows(x, "x");
     const int64_t cols = x.size(-1);
     if (weight.dim() != 1 || weight.size(0) != cols) REFUSE_VALUE("weight has shape ", weight.sizes(), ", expected [", cols, "]");
@@ -109,7 +110,9 @@ py::tuple rms_norm_int8(const Tensor &x, const Tensor &weight, const OptTensor &
     one_device({&x, &weight, residual});
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
-    const Tensor xr = rows_of(x), w = weight.contiguous();
+    // the kernels take the weight in fp32 or in the type of x
+    const Tensor xr = rows_of(x), w = (weight.scalar_type() == x.scalar_type() ? weight : weight.to(at::kFloat)).contiguous();
+    const int wcode = dtype_code(w.scalar_type(), "weight");
     const int64_t rows = xr.size(0);
     const Tensor q = empty_rows(rows, cols, x.device()), scale = at::empty(x.sizes().slice(0, x.dim() - 1), floats(x));
     Tensor rr, total;

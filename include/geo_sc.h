@@ -358,7 +358,7 @@ int geo_sc_pool_act_backward(int planes, int height, int width, const float *x_d
  * a residual), p = r * weight in fp32, q = round_half_even(127 p / max|p|), scale = max|p| / (127 * sqrt(mean(r^2) + eps)),
  * so that q * scale is the normalised row.  q depends on the row alone, not on how it is summed.  residual and
  * sum_out ([rows][cols] dense, receives r; it must not overlap x or residual) come together or are both NULL; weight
- * [cols] of weight_dtype.  A row of zeros has q = 0 and scale = 0; a row whose p or scale is not finite has q = 0 and
+ * [cols] of weight_dtype, fp32 or the type of x.  A row of zeros has q = 0 and scale = 0; a row with a p that is not finite has q = 0 and
  * scale = NaN.  eps >= 0. */
 int geo_sc_rms_norm_int8(long long rows, int cols, int dtype, const void *x_device, long long x_stride,
                          const void *residual_device, long long residual_stride, const void *weight_device,
