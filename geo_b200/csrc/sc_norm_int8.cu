@@ -41,6 +41,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN is kept
     return r;
 }
 
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // VEC products as integers: 127 p / top, half to even; |p| <= top, 1e-30 <= top, finite; inv = 127 / top in fp32.
 // p * inv + 1.5 * 2^23 rounds to an integer whose two's complement is the sum's low byte.  Next to a border h between
 // two integers the sign of 127 p - h top decides, whose products are exact in 64 bits.
@@ -93,36 +99,38 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int by
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_staged(uint32_t at) {   // 16 bytes of shared memory
+    Pack<T, VEC> v;
+    int4 &r = *reinterpret_cast<int4 *>(&v);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+    return v;
+}
+
 // Statistics of a row, joined over its tpr threads (one or more warps of a CTA; part_* have room for two turns).
 struct RowStats {
-    float ss, top;
+    float ss;     // in the row's first warp
+    float top;
     bool again;   // the sum of squares has to be taken again in 64 bits; the same for the whole CTA
 };
 template <bool NORM>
 __device__ __forceinline__ RowStats join_stats(float ss, float top, int tpr, int first, float (*part_ss)[32], float (*part_top)[32], int turn) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = tpr >> 5;
     if (NORM) ss = warp_sum(ss);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     RowStats r;
+    r.top = warp_max_nan(top);
+    r.ss = ss;
     // infinite (or NaN) without a product that is, or vanished without being zero
-    r.again = NORM && top <= 3.402823466e38f && (!(ss <= 3.0e37f) || (ss < 1e-30f && top > 0.f));
+    r.again = NORM && r.top <= 3.402823466e38f && (!(ss <= 3.0e37f) || (ss < 1e-30f && r.top > 0.f));
     if (tpr > 32) {
         if (lane == 0) {
             part_ss[turn][warp] = ss;
-            part_top[turn][warp] = top;
+            part_top[turn][warp] = r.top;
         }
         r.again = __syncthreads_or(r.again);
-        // one partial per lane, joined in the same order by every warp
-        top = part_top[turn][first + (lane & (wpr - 1))];
-        ss = NORM ? part_ss[turn][first + (lane & (wpr - 1))] : 0.f;
-        for (int o = 1; o < wpr; o *= 2) {
-            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        }
+        r.top = warp_max_nan(part_top[turn][first + (lane & (wpr - 1))]);
+        // the sum is wanted by the warp that writes the row's scale
+        if (NORM && warp == first) r.ss = warp_sum(lane < wpr ? part_ss[turn][lane + first] : 0.f);
     }
-    r.ss = ss;
-    r.top = top;
     return r;
 }
 
@@ -147,66 +155,77 @@ __device__ __forceinline__ double join_sum64(double v, int tpr, int first, doubl
     return v;
 }
 
-// tpr threads own a row, VEC values per 16-byte vector, NV vectors of a thread in the stages (longer rows read the rest
-// from memory, twice).  W: the weight's type; without NORM there is none.
+// tpr threads own a row, VEC values per 16-byte vector.  A warp of the row owns 32 * NV neighbouring vectors, a lane
+// every 32nd of them (distances that are known when this is compiled); vectors past 32 * NV per warp are read from memory,
+// twice.  W: the weight's type; without NORM there is none.
 template <typename T, typename W, int NV, bool NORM>
-__global__ void __launch_bounds__(1024) norm_int8_kernel(NormParams pr, int tpr) {
+__global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormParams pr, int tpr) {
     constexpr int VEC = 16 / sizeof(T), STAGES = 3;
     extern __shared__ __align__(16) unsigned char norm_smem[];
     __shared__ float part_ss[2][32], part_top[2][32];
     __shared__ double part64[32];
     const int tid = threadIdx.x % tpr, rpc = blockDim.x / tpr, group = threadIdx.x / tpr, first = group * (tpr >> 5);
-    const int nvec = pr.cols / VEC;
+    const int nvec = pr.cols / VEC, v0 = (tid >> 5) * (32 * NV) + (tid & 31);
     const bool has_res = pr.residual != nullptr;
-    const T *const x = (const T *)pr.x, *const res = (const T *)pr.residual;
-    T *const sum_out = (T *)pr.sum_out;
-    const long long step = (long long)gridDim.x * rpc;
-    // a thread's vectors: [stage][x, residual][NV], blockDim.x vectors apart
-    const uint32_t slot_bytes = blockDim.x * 16, stage_bytes = slot_bytes * NV * (has_res ? 2 : 1);
-    unsigned char *const mine_at = norm_smem + threadIdx.x * 16;
-
-    auto weight_of = [&](int i, float (&w)[VEC]) {
-        if constexpr (NORM) {
-            if constexpr (VEC * sizeof(W) == 32) {   // fp32 weights of 16-bit values: two loads
-                const Pack<W, VEC / 2> a = load_pack<W, VEC / 2>((const W *)pr.weight + i * VEC), b = load_pack<W, VEC / 2>((const W *)pr.weight + i * VEC + VEC / 2);
+    const long long step = (long long)gridDim.x * rpc, start = (long long)blockIdx.x * rpc + group;
+    // a thread's vectors: [stage][x, residual][warp][NV][lane]
+    const uint32_t half = blockDim.x * 16 * NV, stage_bytes = half * (has_res ? 2 : 1);
+    unsigned char *const slots = norm_smem + ((threadIdx.x >> 5) * (32 * NV) + (threadIdx.x & 31)) * 16;
+    bool in[NV];
 #pragma unroll
-                for (int e = 0; e < VEC / 2; e++) {
-                    w[e] = to_float(a.v[e]);
-                    w[VEC / 2 + e] = to_float(b.v[e]);
-                }
-            } else {
-                unpack<VEC>(load_pack<W, VEC>((const W *)pr.weight + i * VEC), w);
+    for (int j = 0; j < NV; j++) {
+        in[j] = v0 + j * 32 < nvec;
+        if (!in[j])   // vectors past the row's end: zeros in every stage, which add nothing to its statistics
+#pragma unroll
+            for (int s = 0; s < STAGES; s++) {
+                *(int4 *)(slots + s * stage_bytes + j * 512) = make_int4(0, 0, 0, 0);
+                if (has_res) *(int4 *)(slots + s * stage_bytes + half + j * 512) = make_int4(0, 0, 0, 0);
             }
+    }
+
+    auto weight_of = [&](const W *at, float (&w)[VEC]) {
+        if constexpr (VEC * sizeof(W) == 32) {   // fp32 weights of 16-bit values: two loads
+            const Pack<W, VEC / 2> a = load_pack<W, VEC / 2>(at), b = load_pack<W, VEC / 2>(at + VEC / 2);
+#pragma unroll
+            for (int e = 0; e < VEC / 2; e++) {
+                w[e] = to_float(a.v[e]);
+                w[VEC / 2 + e] = to_float(b.v[e]);
+            }
+        } else {
+            unpack<VEC>(load_pack<W, VEC>(at), w);
         }
     };
-    auto ask = [&](long long row, int stage) {
+    const T *next_x = (const T *)pr.x + start * pr.x_stride + v0 * VEC, *next_r = (const T *)pr.residual + start * pr.res_stride + v0 * VEC;
+    auto ask = [&](long long row, int stage) {   // the rows in turn
         if (row < pr.rows) {
-            const T *px = x + row * pr.x_stride, *pq = res + row * pr.res_stride;
-            const uint32_t dst = smem_u32(mine_at) + stage * stage_bytes;
+            const uint32_t dst = smem_u32(slots) + stage * stage_bytes;
 #pragma unroll
             for (int j = 0; j < NV; j++)
-                if (tid + j * tpr < nvec) {
-                    copy_async(dst + j * slot_bytes, px + (tid + j * tpr) * VEC, 16);
-                    if (has_res) copy_async(dst + (NV + j) * slot_bytes, pq + (tid + j * tpr) * VEC, 16);
+                if (in[j]) {
+                    copy_async(dst + j * 512, next_x + j * 32 * VEC, 16);
+                    if (has_res) copy_async(dst + half + j * 512, next_r + j * 32 * VEC, 16);
                 }
         }
         copy_commit();
+        next_x += step * pr.x_stride;
+        next_r += step * pr.res_stride;
     };
-    const long long start = (long long)blockIdx.x * rpc;
-    ask(start + group, 0);
-    ask(start + step + group, 1);
+    ask(start, 0);
+    ask(start + step, 1);
     int turn = 0, stage = 0;
+    T *sum_at = (T *)pr.sum_out + start * pr.cols + v0 * VEC;
+    int8_t *q_at = pr.q + start * pr.q_stride + v0 * VEC;
+    const W *const w_at = (const W *)pr.weight + v0 * VEC;
     // every thread of a CTA makes the same number of turns; rows past the end take part in the barriers only
-    for (long long base = start; base < pr.rows; base += step, turn ^= 1) {
-        const long long row = base + group;
-        const int mine = row < pr.rows ? nvec : 0;
+    for (long long row = start; row - group < pr.rows; row += step, turn ^= 1) {
+        const bool live = row < pr.rows;
         ask(row + 2 * step, stage == 0 ? 2 : stage - 1);
         copy_wait<2>();
         float p[NV][VEC], ss = 0.f, top = 0.f;
-        auto take = [&](const Pack<T, VEC> &v, int i, float (&pv)[VEC]) {
+        auto take = [&](const Pack<T, VEC> &v, const W *at, float (&pv)[VEC]) {
             float r[VEC], wv[VEC];
             unpack<VEC>(v, r);
-            weight_of(i, wv);
+            if constexpr (NORM) weight_of(at, wv);
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
                 if (NORM) ss = fmaf(r[e], r[e], ss);
@@ -216,63 +235,67 @@ __global__ void __launch_bounds__(1024) norm_int8_kernel(NormParams pr, int tpr)
         };
         // a vector from memory: past the stages' part of the row, or once more
         auto far = [&](int i, bool write) {
-            Pack<T, VEC> v = load_pack<T, VEC>(x + row * pr.x_stride + (long long)i * VEC);
+            Pack<T, VEC> v = load_pack<T, VEC>((const T *)pr.x + row * pr.x_stride + (long long)i * VEC);
             if (has_res) {
-                add_pack<T, VEC>(v, load_pack<T, VEC>(res + row * pr.res_stride + (long long)i * VEC));
-                if (write) store_pack<T, VEC>(sum_out + row * pr.cols + (long long)i * VEC, v);
+                add_pack<T, VEC>(v, load_pack<T, VEC>((const T *)pr.residual + row * pr.res_stride + (long long)i * VEC));
+                if (write) store_pack<T, VEC>((T *)pr.sum_out + row * pr.cols + (long long)i * VEC, v);
             }
             return v;
         };
-        const unsigned char *const at = mine_at + stage * stage_bytes;
+        const uint32_t at = smem_u32(slots) + stage * stage_bytes;
 #pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (tid + j * tpr < mine) {
-                Pack<T, VEC> v = *(const Pack<T, VEC> *)(at + j * slot_bytes);
-                if (has_res) {
-                    add_pack<T, VEC>(v, *(const Pack<T, VEC> *)(at + (NV + j) * slot_bytes));
-                    store_pack<T, VEC>(sum_out + row * pr.cols + (tid + j * tpr) * VEC, v);
-                }
-                take(v, tid + j * tpr, p[j]);
+        for (int j = 0; j < NV; j++) {
+            Pack<T, VEC> v = load_staged<T, VEC>(at + j * 512);
+            if (has_res) {
+                add_pack<T, VEC>(v, load_staged<T, VEC>(at + half + j * 512));
+                if (in[j] && live) store_pack<T, VEC>(sum_at + j * 32 * VEC, v);
             }
-        for (int i = tid + NV * tpr; i < mine; i += tpr) {
+            take(v, in[j] ? w_at + j * 32 * VEC : (const W *)pr.weight, p[j]);
+        }
+        for (int i = tid + NV * tpr; i < nvec && live; i += tpr) {
             float pv[VEC];
-            take(far(i, true), i, pv);
+            take(far(i, true), (const W *)pr.weight + (long long)i * VEC, pv);
         }
         stage = stage == 2 ? 0 : stage + 1;
 
         const RowStats st = join_stats<NORM>(ss, top, tpr, first, part_ss, part_top, turn);
         double total = 0;
         if (NORM && st.again) {
-            for (int i = tid; i < mine; i += tpr) {
+            for (int i = tid; i < nvec && live; i += tpr) {
                 float r[VEC];
                 unpack<VEC>(far(i, false), r);
                 for (int e = 0; e < VEC; e++) total += (double)r[e] * (double)r[e];
             }
             total = join_sum64(total, tpr, first, part64);
         }
-        if (mine == 0) continue;
-        if (tid == 0) pr.scale[row] = row_scale<NORM>(st, total, pr.cols, pr.eps);
-
-        const bool zero = !(st.top <= 3.402823466e38f) || st.top == 0.f;
-        // products below the normal range of a reciprocal: the integers are those of 2^64 times the row
-        const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = 127.f / lifted;
-        int8_t *q = pr.q + row * pr.q_stride;
-        auto give = [&](float (&pv)[VEC], int i) {
-            Pack<int8_t, VEC> o = {};
-            if (lift != 1.f)
+        if (live) {
+            if (tid == 0) pr.scale[row] = row_scale<NORM>(st, total, pr.cols, pr.eps);
+            const bool fine = st.top <= 3.402823466e38f;
+            // products below the normal range of a reciprocal: the integers are those of 2^64 times the row; a row with a
+            // product that is not finite, or of zeros, has zeros
+            const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift;
+            const float inv = fine && st.top > 0.f ? 127.f / lifted : 0.f;
+            const bool plain = fine && lift == 1.f;
+            if (!plain)
 #pragma unroll
-                for (int e = 0; e < VEC; e++) pv[e] *= lift;
-            if (!zero) o = round_pack<VEC>(pv, lifted, inv);
-            store_pack<int8_t, VEC>(q + (long long)i * VEC, o);
-        };
+                for (int j = 0; j < NV; j++)
 #pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (tid + j * tpr < mine) give(p[j], tid + j * tpr);
-        for (int i = tid + NV * tpr; i < mine; i += tpr) {
-            float pv[VEC];
-            take(far(i, false), i, pv);
-            give(pv, i);
+                    for (int e = 0; e < VEC; e++) p[j][e] = fine ? p[j][e] * lift : 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const Pack<int8_t, VEC> o = round_pack<VEC>(p[j], lifted, inv);
+                if (in[j]) store_pack<int8_t, VEC>(q_at + j * 32 * VEC, o);
+            }
+            for (int i = tid + NV * tpr; i < nvec; i += tpr) {
+                float pv[VEC];
+                take(far(i, false), (const W *)pr.weight + (long long)i * VEC, pv);
+                if (!plain)
+                    for (int e = 0; e < VEC; e++) pv[e] = fine ? pv[e] * lift : 0.f;
+                store_pack<int8_t, VEC>(pr.q + row * pr.q_stride + (long long)i * VEC, round_pack<VEC>(pv, lifted, inv));
+            }
         }
+        sum_at += step * pr.cols;
+        q_at += step * pr.q_stride;
     }
     copy_wait<0>();
 }
@@ -371,7 +394,7 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
 constexpr int NORM_SMEM = 200 * 1024;   // of an SM's 227 KB, shared by its CTAs
 
 template <typename T, typename W, int NV, bool NORM> int launch_norm_nv(const NormParams &p, int tpr, cudaStream_t s) {
-    const int threads = tpr < 256 && p.rows > 1 ? 256 : tpr, rpc = threads / tpr;
+    const int threads = tpr < 128 && p.rows > 1 ? 128 : tpr, rpc = threads / tpr;
     const int smem = threads * 16 * NV * (p.residual ? 2 : 1) * 3;
     static PerDeviceOnce once;
     int rc = per_device_once(once, []() -> int {
@@ -379,8 +402,9 @@ template <typename T, typename W, int NV, bool NORM> int launch_norm_nv(const No
         return GEO_SC_OK;
     });
     if (rc) return rc;
-    // as many CTAs as fit 1024 threads of 64 registers and the stages on every SM
-    const long long need = (p.rows + rpc - 1) / rpc, most = (long long)sm_count() * max(1, min(1024 / threads, NORM_SMEM / smem));
+    // as many CTAs as fit every SM's registers and the stages
+    const int per_sm = max(1, min((NV == 4 ? 512 : 1024) / threads, NORM_SMEM / smem));
+    const long long need = (p.rows + rpc - 1) / rpc, most = (long long)sm_count() * per_sm;
     norm_int8_kernel<T, W, NV, NORM><<<(unsigned)(need < most ? need : most), threads, smem, s>>>(p, tpr);
     GEO_CUDA_CHECK(cudaGetLastError());
     return GEO_SC_OK;
@@ -392,11 +416,15 @@ template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p
     const bool wide = p.cols % VEC == 0 && aligned_to(p.x, 16) && p.x_stride % VEC == 0 && (!p.residual || (aligned_to(p.residual, 16) && p.res_stride % VEC == 0)) &&
                       (!p.sum_out || aligned_to(p.sum_out, 16)) && aligned_to(p.q, VEC) && p.q_stride % VEC == 0 && (!NORM || aligned_to(p.weight, 16));
     if (wide) {
-        // few rows: one vector per thread, the shortest way through a row; many: two, for half the reductions
-        const int nvec = p.cols / VEC, want = p.rows < 2LL * sm_count() ? nvec : (nvec + 1) / 2;
+        // few rows: one vector per thread, the shortest way through a row; many: four, for a quarter of the reductions
+        // (16384 rows of 8192 fp16 values: with two vectors 220 us, of 320 instructions per vector two thirds per row)
+        const int nvec = p.cols / VEC;
+        const bool few = p.rows < 2LL * sm_count() && nvec <= 1024;
         int tpr = 32;
-        while (tpr < 1024 && tpr < want) tpr *= 2;
-        return nvec <= tpr ? launch_norm_nv<T, W, 1, NORM>(p, tpr, s) : launch_norm_nv<T, W, 2, NORM>(p, tpr, s);
+        while (tpr < (few ? 1024 : 512) && tpr < (few ? nvec : (nvec + 3) / 4)) tpr *= 2;
+        if (nvec <= tpr) return launch_norm_nv<T, W, 1, NORM>(p, tpr, s);
+        if (nvec <= 2 * tpr) return launch_norm_nv<T, W, 2, NORM>(p, tpr, s);
+        return launch_norm_nv<T, W, 4, NORM>(p, tpr, s);
     }
     int threads = 64;
     while (threads < 1024 && threads * 8 < p.cols) threads *= 2;

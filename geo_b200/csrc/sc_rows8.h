@@ -19,11 +19,21 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 // N values of T as one load or store (N * sizeof(T) is 16, 8 or 4 bytes, or N = 1).
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };
 
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { using type = int4; };
+template <> struct Raw<8> { using type = int2; };
+template <> struct Raw<4> { using type = int; };
+template <> struct Raw<2> { using type = short; };
+template <> struct Raw<1> { using type = signed char; };
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
-    return *reinterpret_cast<const Pack<T, N> *>(p);
+    using R = typename Raw<sizeof(Pack<T, N>)>::type;
+    Pack<T, N> v;
+    *reinterpret_cast<R *>(&v) = *reinterpret_cast<const R *>(p);
+    return v;
 }
 template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &v) {
-    *reinterpret_cast<Pack<T, N> *>(p) = v;
+    using R = typename Raw<sizeof(Pack<T, N>)>::type;
+    *reinterpret_cast<R *>(p) = *reinterpret_cast<const R *>(&v);
 }
 
 // Packs to and from fp32, two 16-bit values per instruction.
@@ -47,13 +57,10 @@ template <int N> __device__ __forceinline__ void unpack(const Pack<__half, N> &v
     if constexpr (N == 1) {
         f[0] = __half2float(v.v[0]);
     } else {
-        const __half2 *w = reinterpret_cast<const __half2 *>(&v);
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
 #pragma unroll
-        for (int e = 0; e < N / 2; e++) {
-            const float2 t = __half22float2(w[e]);
-            f[2 * e] = t.x;
-            f[2 * e + 1] = t.y;
-        }
+        for (int e = 0; e < N / 2; e++)
+            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}\n" : "=f"(f[2 * e]), "=f"(f[2 * e + 1]) : "r"(w[e]));
     }
 }
 template <int N> __device__ __forceinline__ void pack(Pack<float, N> &v, const float (&f)[N]) {
@@ -64,18 +71,18 @@ template <int N> __device__ __forceinline__ void pack(Pack<__nv_bfloat16, N> &v,
     if constexpr (N == 1) {
         v.v[0] = __float2bfloat16_rn(f[0]);
     } else {
-        __nv_bfloat162 *w = reinterpret_cast<__nv_bfloat162 *>(&v);
+        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
-        for (int e = 0; e < N / 2; e++) w[e] = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+        for (int e = 0; e < N / 2; e++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(f[2 * e + 1]), "f"(f[2 * e]));
     }
 }
 template <int N> __device__ __forceinline__ void pack(Pack<__half, N> &v, const float (&f)[N]) {
     if constexpr (N == 1) {
         v.v[0] = __float2half_rn(f[0]);
     } else {
-        __half2 *w = reinterpret_cast<__half2 *>(&v);
+        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
-        for (int e = 0; e < N / 2; e++) w[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+        for (int e = 0; e < N / 2; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(f[2 * e + 1]), "f"(f[2 * e]));
     }
 }
 // Four signed bytes as floats: a byte b + 128 in the low mantissa of 2^23 is the float 2^23 + 128 + b, exactly.
