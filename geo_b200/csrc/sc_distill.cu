@@ -5,17 +5,25 @@
 //   loss = weight * T^2 * sum_k p_k (log p_k - log q_{index_k})
 //   d loss / d z_j = weight * T * (q_j - sum of the p_k whose index is j)
 // Entries with a negative index are padding, an entry of -inf has p = 0.  A row without a single entry above -inf, or
-// of weight 0, has loss 0 and gradient 0, and its logits are not read.  An index at or past the vocabulary, or a
+// of weight 0, has loss 0 and gradient 0, whatever its logits are.  An index at or past the vocabulary, or a
 // teacher's logit that is NaN or +inf, makes the row's loss and gradient NaN; nothing is read or written through it.
 //
-// With m the row's largest logit, S = sum_j exp((z_j - m) / T): q_j = exp((z_j - m) / T) / S.  The difference z - m is
-// taken before it is scaled, so that the terms which carry the sum have small arguments and small errors.  Every thread
-// keeps a running maximum and a running sum (rescaled when the maximum grows) in one pass over the row; these pairs are
-// joined in a fixed order.  Sums over the entries and over the rows are taken in 64 bits.
+// In base 2, with c = log2(e) / T, m the row's largest logit, the reference r = fl(m c) and S = sum_j 2^(z_j c - r):
+// q_j = 2^(z_j c - r) / S.  The argument is one fused multiply-add, rounded relative to itself, so the terms which carry
+// the sum have small errors; that r is rounded does not matter, because every term and every partial sum is taken
+// against a reference that is kept as it is.  Past |m c| = 2^30 (rows masked by the type's lowest value throughout) that
+// rounding is too coarse; there two different values of any of the types are at least 64 apart in the exponent, and
+// logits other than m count as -inf, m as 0.
+// Sums over the entries and over the rows are joined in a fixed order, the
+// loss in 64 bits.
 //
-// What bounds it: HBM.  One read of the logits and, with the gradient, one write: the second pass of a team over its row
-// comes from L2.  A team of one warp owns a row of a small vocabulary, a CTA one of a larger vocabulary, and where
-// there are fewer rows than SMs a cluster of CTAs shares a row and joins the pairs over distributed shared memory.
+// What bounds it: HBM, one read of the logits and, with the gradient, one write.  A team copies its share of a row into
+// shared memory (cp.async, all of it asked for at once; a thread copies the vectors that it computes), so the largest
+// logit, the sum and the gradient read memory once.  Teams: a warp, a CTA of 128 or 256 threads, or a cluster of up to
+// eight CTAs of 256, whichever holds the row with sixteen 16-byte vectors per thread (more threads where there are few
+// rows); what a cluster of eight cannot hold is read again.  Few warps with many vectors each, because what a row costs
+// a warp besides its vectors is the same for any number.  A warp of its own takes the teacher's entries of a CTA's row
+// while the logits are on their way, and the loss while the gradient is written.
 #include <cooperative_groups.h>
 
 #include "sc_rows8.h"
@@ -26,8 +34,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int DISTILL_MAX_TOP = 512;
-constexpr int DISTILL_WARP_VOCAB = 1024;   // vocabularies up to this: one warp per row
+constexpr int DISTILL_HOLD = 16;  // 16-byte vectors of a row that a thread holds
 constexpr float NEG_INF = -INFINITY;
+constexpr float FAR = 1073741824.f;   // 2^30
 
 struct DistillParams {
     const void *logits, *indices, *teacher;
@@ -48,37 +57,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
-// Joins per-thread values of a team of TEAM threads (a warp, or the whole CTA); every thread gets the result.
-template <int TEAM> struct Team {
-    float *buf;   // 32 floats and 32 doubles' room, CTA teams only
-    __device__ float max(float v) {
-        v = warp_max(v);
-        if (TEAM == 32) return v;
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = buf[0];
-        for (int i = 1; i < TEAM / 32; i++) v = fmaxf(v, buf[i]);
-        return v;
-    }
-    template <typename V> __device__ V sum(V v) {
-        v = warp_sum(v);
-        if (TEAM == 32) return v;
-        V *b = (V *)buf;
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = b[0];
-        for (int i = 1; i < TEAM / 32; i++) v += b[i];
-        return v;
-    }
-    __device__ bool any(bool v) { return TEAM == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
-    __device__ void sync() {
-        if (TEAM == 32) __syncwarp();
-        else __syncthreads();
-    }
-};
 
 __device__ __forceinline__ float teacher_at(const DistillParams &p, long long i) {
     if (p.teacher_dtype == GEO_SC_DTYPE_F32) return ((const float *)p.teacher)[i];
@@ -103,182 +81,352 @@ template <typename T> __device__ __forceinline__ Slice slice_of(const T *row, in
     return s;
 }
 
+// What terms are taken against where r is the largest z c: 0 far below, where they are 0 (or NaN) and not the exponential
+// of a rounding or of -inf + inf.
+__device__ __forceinline__ float base_of(float r) { return r < -FAR ? 0.f : r; }
+// A sum taken against base_of(from), as one against `to` >= from.
+__device__ __forceinline__ float moved(float sum, float from, float to) { return from < -FAR ? sum : sum * ex2(from - to); }
+
+constexpr int team_threads(int team) { return team == 32 ? 128 : team + 32; }   // four warps with a row each; or a team and the entries' warp
+constexpr int team_blocks(int team) { return team == 32 ? 8 : 896 / team; }         // that registers are left for, of an SM
+constexpr int DISTILL_SMEM = 200 * 1024;   // of an SM's 227 KB
+// a team's shared memory: 20 bytes per entry, the table that finds entries of the same index, then the team's vectors
+__host__ __device__ inline int table_slots(int top) {
+    int n = 32;
+    while (n < 2 * top) n *= 2;
+    return n;
+}
+__host__ __device__ inline int entry_room(int top) { return (top * 20 + table_slots(top) * 4 + 15) / 16 * 16; }
+
+// The teacher's entries of a row in shared memory, taken by one warp.
+struct Entries {
+    int *idx;        // -1: no part
+    float *prob;     // exp((t - largest t) / T)
+    float *diff;     // (t - largest t) / T
+    float *own;      // the student's logit
+    float *merged;   // the probability of an index, by its first entry of those in [from, to); else -1
+    int *table;
+    int slots;
+};
+// 0: a row with entries, 1: without (or of weight 0), 2: with a bad entry.
+template <typename T, bool GRAD>
+__device__ __forceinline__ int take_entries(const DistillParams &pr, const Entries &en, long long row, const T *z, float w, float inv_t, int from, int to, float &psum) {
+    const int lane = threadIdx.x & 31;
+    float tmax = NEG_INF;
+    bool bad = false;
+    if (GRAD)
+        for (int i = lane; i < en.slots; i += 32) en.table[i] = -1;
+    for (int k = lane; k < pr.top; k += 32) {
+        const long long at = row * pr.top + k;
+        const long long j = pr.index64 ? ((const long long *)pr.indices)[at] : ((const int *)pr.indices)[at];
+        const float t = teacher_at(pr, at);
+        const bool use = j >= 0, fits = use && j < pr.vocab;
+        bad |= use && (!fits || !(t < INFINITY));
+        en.idx[k] = fits ? (int)j : -1;
+        en.own[k] = fits ? to_float(z[j]) : 0.f;
+        en.diff[k] = use ? t : NEG_INF;
+        if (use) tmax = fmaxf(tmax, t);
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    tmax = warp_max(tmax);
+    if (w == 0.f || (!bad && tmax == NEG_INF)) return 1;
+    if (bad) return 2;
+    psum = 0.f;
+    bool twice = false;
+    __syncwarp();   // the table is clear
+    for (int k = lane; k < pr.top; k += 32) {
+        const float d = (en.diff[k] - tmax) * inv_t, e = expf(d);
+        en.diff[k] = d;
+        en.prob[k] = e;
+        psum += e;
+        const int j = en.idx[k];
+        if (GRAD && j >= 0) {   // open addressing; at most half of the slots are ever taken
+            for (int i = (unsigned)j * 2654435769u >> 16;; i++) {
+                const int was = atomicCAS(&en.table[i & (en.slots - 1)], -1, j);
+                twice |= was == j;
+                if (was == -1 || was == j) break;
+            }
+        }
+    }
+    psum = warp_sum(psum);
+    if (GRAD) {
+        twice = __any_sync(0xffffffffu, twice);
+        __syncwarp();
+        for (int k = lane; k < pr.top; k += 32) {
+            const int j = en.idx[k];
+            bool first = j >= from && j < to;
+            float p = en.prob[k];
+            if (twice && first) {
+                p = 0.f;
+                for (int i = 0; i < pr.top; i++)
+                    if (en.idx[i] == j) {
+                        p += en.prob[i];
+                        first &= i >= k;
+                    }
+            }
+            en.merged[k] = first ? p / psum : -1.f;
+        }
+    }
+    return 0;
+}
+
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER>
-__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM) distill_kernel(DistillParams pr) {
-    constexpr int VEC = 16 / sizeof(T);
+__global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill_kernel(DistillParams pr, int team_bytes) {
+    constexpr int VEC = 16 / sizeof(T), WARPS = TEAM / 32, HOP = TEAM * 16;   // bytes between a thread's vectors
     extern __shared__ __align__(16) unsigned char distill_smem[];
-    __shared__ __align__(16) float reduce_buf[64];
-    __shared__ float2 pair;   // this CTA's (m, S), read by the other CTAs of the cluster
-    const int tid = TEAM == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int slot = TEAM == 32 ? threadIdx.x >> 5 : 0;
+    __shared__ float2 part[8];
+    __shared__ float2 pair;   // this CTA's (largest logit, sum), read by the other CTAs of the cluster
+    __shared__ int row_state;
+    __shared__ float row_psum;
+    const int lane = threadIdx.x & 31, warp = TEAM == 32 ? 0 : threadIdx.x >> 5, slot = TEAM == 32 ? threadIdx.x >> 5 : 0;
+    const int tid = TEAM == 32 ? lane : threadIdx.x;
+    const bool scribe = TEAM == 32 || warp == WARPS, streams = TEAM == 32 || warp < WARPS;   // who takes the entries, who the logits
     int rank = 0, ranks = 1;
     if (CLUSTER) {
         rank = (int)cg::this_cluster().block_rank();
         ranks = (int)cg::this_cluster().num_blocks();
     }
-    const long long row = TEAM == 32 ? (long long)blockIdx.x * (blockDim.x / 32) + slot : (long long)(blockIdx.x / ranks);
-    if (TEAM == 32 && row >= pr.rows) return;
-    Team<TEAM> team{reduce_buf};
-    int *const idx = (int *)distill_smem + (size_t)slot * 2 * pr.top;   // an entry's index, -1 where it has no part
-    float *const prob = (float *)(idx + pr.top);
-
-    float up = 1.f;
-    if (!STATS) {
-        up = pr.upstream[pr.upstream_rows ? row : 0];
-        if (pr.skip_one && up == 1.f) return;
-    }
-    const T *z = (const T *)pr.logits + row * pr.stride;
-    T *grad = GRAD ? (T *)pr.grad + row * (long long)pr.vocab : nullptr;
-    const float w = pr.weight ? pr.weight[row] : 1.f;
-    const Slice sl = slice_of(z, pr.vocab, rank, ranks);
     const bool last = rank == ranks - 1;
+    auto team_sync = [&]() {
+        if (TEAM == 32) __syncwarp();
+        else __syncthreads();
+    };
+    Entries en;
+    en.idx = (int *)(distill_smem + slot * team_bytes);
+    en.prob = (float *)(en.idx + pr.top);
+    en.diff = en.prob + pr.top;
+    en.own = en.diff + pr.top;
+    en.merged = en.own + pr.top;
+    en.table = (int *)(en.merged + pr.top);
+    en.slots = table_slots(pr.top);
+    const uint32_t held = smem_u32(en.idx) + entry_room(pr.top) + tid * 16;   // a thread's vectors
+    const float inv_t = 1.f / pr.temperature, c = 1.4426950408889634f * inv_t;
+    auto scaled = [&](float v) { return __fmul_rn(v, c); };   // a reference: rounded, never part of a fused multiply-add
 
-    // the teacher's entries
-    const float inv_t = 1.f / pr.temperature;
-    float tmax = NEG_INF;
-    bool bad = false;
-    for (int k = tid; k < pr.top; k += TEAM) {
-        const long long at = row * pr.top + k;
-        const long long j = pr.index64 ? ((const long long *)pr.indices)[at] : ((const int *)pr.indices)[at];
-        const float t = teacher_at(pr, at);
-        const bool use = j >= 0;
-        if (use && (j >= pr.vocab || !(t < INFINITY))) bad = true;
-        idx[k] = use && j < pr.vocab ? (int)j : -1;
-        prob[k] = use ? t : NEG_INF;
-        if (use) tmax = fmaxf(tmax, t);
-    }
-    bad = team.any(bad);
-    tmax = team.max(tmax);
-    const bool dead = (!bad && tmax == NEG_INF) || w == 0.f;
-    if (dead || bad) {   // the same for every CTA of a cluster
-        const float v = dead ? 0.f : __int_as_float(0x7fc00000);
-        if (STATS && rank == 0 && tid == 0) {
-            pr.row_loss[row] = v;
-            pr.stats[row] = make_float2(0.f, 1.f);
+    const long long teams = TEAM == 32 ? (long long)gridDim.x * 4 : gridDim.x / ranks;
+    for (long long row = TEAM == 32 ? (long long)blockIdx.x * 4 + slot : blockIdx.x / ranks; row < pr.rows; row += teams) {
+        float up = 1.f;
+        if (!STATS) {
+            up = pr.upstream[pr.upstream_rows ? row : 0];
+            if (pr.skip_one && up == 1.f) continue;
         }
-        if (GRAD) {
-            const int from = rank == 0 ? 0 : sl.head + sl.v0 * VEC, to = last ? pr.vocab : sl.head + sl.v1 * VEC;
-            for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(v);
-        }
-        return;
-    }
-    float psum = 0.f;
-    for (int k = tid; k < pr.top; k += TEAM) {
-        const float e = expf((prob[k] - tmax) * inv_t);   // an entry's exponential; divided by the sum when used
-        if (!STATS) prob[k] = e;
-        psum += e;
-    }
-    psum = team.sum(psum);
-    const float inv_psum = 1.f / psum;
+        const T *const z = (const T *)pr.logits + row * pr.stride;
+        T *const grad = GRAD ? (T *)pr.grad + row * (long long)pr.vocab : nullptr;
+        const Slice sl = slice_of(z, pr.vocab, rank, ranks);
+        const T *const zv = z + sl.head;
+        const float w = pr.weight ? pr.weight[row] : 1.f;
+        const int from = rank == 0 ? 0 : sl.head + sl.v0 * VEC, to = last ? pr.vocab : sl.head + sl.v1 * VEC;
 
-    const float c = 1.4426950408889634f * inv_t;
-    float m, S;
-    if (STATS) {
-        m = NEG_INF;
-        S = 0.f;
-        auto take = [&](float v) {
-            if (v > m) {
-                S *= ex2((m - v) * c);
-                m = v;
+        // The same number of vectors for every lane of a warp; those past the slice are -inf.  From v_far on: read again.
+        int n_held = 0;
+        const int v_first = sl.v0 + tid, v_far = v_first + DISTILL_HOLD * TEAM;
+        // the values before the first and after the last vector, one per thread
+        int r_at = -1;
+        float r_value = 0.f;
+        if (streams) {
+            n_held = min(max(0, sl.v1 - (sl.v0 + warp * 32) + TEAM - 1) / TEAM, DISTILL_HOLD);
+            const T *src = zv + (long long)v_first * VEC;
+            uint32_t dst = held;
+            for (int h = 0; h < n_held; h++, src += TEAM * VEC, dst += HOP)
+                if (v_first + h * TEAM < sl.v1) copy_async(dst, src, 16);
+            if (n_held > 0 && v_first + (n_held - 1) * TEAM >= sl.v1) {
+                Pack<T, VEC> none;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) none.v[e] = from_float<T>(NEG_INF);
+                store_staged<T, VEC>(held + (n_held - 1) * HOP, none);
             }
-            S += ex2((v - (m == NEG_INF ? 0.f : m)) * c);
+            const int heads = rank == 0 ? sl.head : 0, ragged = heads + (last ? pr.vocab - sl.tail : 0);
+            r_at = tid < heads ? tid : tid < ragged ? sl.tail + tid - heads : -1;
+            if (r_at >= 0) r_value = to_float(z[r_at]);
+            copy_commit();
+        }
+        int state = 0;
+        float psum = 1.f;
+        if (scribe) {
+            state = take_entries<T, GRAD>(pr, en, row, z, w, inv_t, from, to, psum);
+            if (TEAM > 32 && lane == 0) {
+                row_state = state;
+                row_psum = psum;
+            }
+            __syncwarp();
+        }
+        if (streams) copy_wait<0>();
+
+        float m = 0.f, sum = 0.f;
+        bool flat = false;   // m c out of range: a logit is either m or nothing
+        auto seen = [&](float v) { return !flat ? v : v == m ? 0.f : NEG_INF; };
+        auto flatten = [&]() {
+            flat = true;
+            for (int h = 0; h < n_held; h++) {
+                float f[VEC];
+                Pack<T, VEC> v = load_staged<T, VEC>(held + h * HOP);
+                unpack<VEC>(v, f);
+#pragma unroll
+                for (int e = 0; e < VEC; e++) f[e] = seen(f[e]);
+                pack<VEC>(v, f);
+                store_staged<T, VEC>(held + h * HOP, v);
+            }
+            r_value = seen(r_value);
         };
-        if (rank == 0)
-            for (int j = tid; j < sl.head; j += TEAM) take(to_float(z[j]));
-        if (last)
-            for (int j = sl.tail + tid; j < pr.vocab; j += TEAM) take(to_float(z[j]));
-        const T *zv = z + sl.head;
+        auto out_of_range = [&]() { return fabsf(m) <= 3.402823466e38f && !(fabsf(scaled(m)) <= FAR); };
+        // Largest logit and sum of the warp.  A thread's reference is the first largest value that it meets, and moves only
+        // for one that is 2^32 times as probable (some lane would move it at nearly every vector otherwise); sums stay far
+        // below 2^127.
+        auto warp_stats = [&](float &most, float &total) {
+            float top = r_at >= 0 ? r_value : NEG_INF;
+            if (n_held > 0) top = fmaxf(top, pack_max<VEC>(load_staged<T, VEC>(held)));
+            float ref = scaled(top), base = base_of(ref), s0 = r_at >= 0 ? ex2(fmaf(r_value, c, -base)) : 0.f, s1 = 0.f;
+            auto add = [&](const float (&f)[VEC], float large) {
+                top = fmaxf(top, large);
+                if (scaled(large) > ref + 32.f) {
+                    const float to_ref = scaled(large);
+                    s0 = moved(s0, ref, to_ref);
+                    s1 = moved(s1, ref, to_ref);
+                    ref = to_ref;
+                    base = base_of(ref);
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    s0 += ex2(fmaf(f[e], c, -base));
+                    s1 += ex2(fmaf(f[e + 1], c, -base));
+                }
+            };
 #pragma unroll 4
-        for (int i = sl.v0 + tid; i < sl.v1; i += TEAM) {
-            const Pack<T, VEC> v = load_pack<T, VEC>(zv + (long long)i * VEC);
-            float f[VEC], top = NEG_INF;
+            for (int h = 0; h < n_held; h++) {
+                const Pack<T, VEC> v = load_staged<T, VEC>(held + h * HOP);
+                float f[VEC];
+                unpack<VEC>(v, f);
+                add(f, pack_max<VEC>(v));
+            }
+            for (int i = v_far; i < sl.v1; i += TEAM) {
+                float f[VEC], large = NEG_INF;
+                unpack<VEC>(load_pack<T, VEC>(zv + (long long)i * VEC), f);
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                f[e] = to_float(v.v[e]);
-                top = fmaxf(top, f[e]);
+                for (int e = 0; e < VEC; e++) {
+                    f[e] = seen(f[e]);
+                    large = fmaxf(large, f[e]);
+                }
+                add(f, large);
             }
-            if (top > m) {
-                S *= ex2((m - top) * c);
-                m = top;
+            most = warp_max(top);
+            total = warp_sum(moved(s0 + s1, ref, scaled(most)));
+        };
+
+        if (STATS) {
+            for (;;) {
+                float most = NEG_INF;
+                if (streams) warp_stats(most, sum);
+                if (TEAM > 32) {
+                    if (streams && lane == 0) part[warp] = make_float2(most, sum);
+                    __syncthreads();
+                    const float2 v = part[lane & (WARPS - 1)];
+                    most = warp_max(v.x);
+                    sum = warp_sum(lane < WARPS ? moved(v.y, scaled(v.x), scaled(most)) : 0.f);
+                }
+                if (CLUSTER) {
+                    cg::cluster_group cluster = cg::this_cluster();
+                    if (tid == 0) pair = make_float2(most, sum);
+                    cluster.sync();
+                    const float2 v = *cluster.map_shared_rank(&pair, lane & (ranks - 1));
+                    cluster.sync();   // nobody leaves, or writes its next pair, while it may still be read
+                    most = warp_max(v.x);
+                    sum = warp_sum(lane < ranks ? moved(v.y, scaled(v.x), scaled(most)) : 0.f);
+                }
+                if (flat) break;
+                m = most;
+                if (!out_of_range()) break;
+                if (streams) flatten();
+                flat = true;
+                team_sync();   // before the next partials
             }
-            const float base = m == NEG_INF ? 0.f : m;
+            if (m == NEG_INF) sum = __int_as_float(0x7fc00000);   // no logit above -inf: no distribution
+        } else {
+            team_sync();
+            m = pr.stats[row].x;
+            sum = pr.stats[row].y;
+            if (out_of_range()) {
+                if (streams) flatten();
+                flat = true;
+            }
+        }
+        if (TEAM > 32) {
+            state = row_state;
+            psum = row_psum;
+        }
+        const float ref = flat ? 0.f : scaled(m);
+        const bool wide = GRAD && ((uintptr_t)(grad + sl.head) & 15) == 0;
+
+        if (state) {   // the same for every CTA of a cluster
+            const float v = state == 1 ? 0.f : __int_as_float(0x7fc00000);
+            if (STATS && rank == 0 && tid == 0) {
+                pr.row_loss[row] = v;
+                pr.stats[row] = make_float2(0.f, 1.f);
+            }
+            if (GRAD && streams) {
+                Pack<T, VEC> o;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) S += ex2((f[e] - base) * c);
-        }
-        float top = team.max(m);
-        S = team.sum(S * (m == NEG_INF ? (S == 0.f ? 0.f : 1.f) : ex2((m - top) * c)));
-        m = top;
-        if (CLUSTER) {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (tid == 0) pair = make_float2(m, S);
-            cluster.sync();
-            top = NEG_INF;
-            for (int r = 0; r < ranks; r++) top = fmaxf(top, cluster.map_shared_rank(&pair, r)->x);
-            S = 0.f;
-            for (int r = 0; r < ranks; r++) {
-                const float2 v = *cluster.map_shared_rank(&pair, r);
-                S += v.y * (v.x == NEG_INF ? (v.y == 0.f ? 0.f : 1.f) : ex2((v.x - top) * c));
-            }
-            m = top;
-            cluster.sync();   // nobody leaves while its pair may still be read
-        }
-        if (m == NEG_INF) S = __int_as_float(0x7fc00000);   // no logit above -inf: no distribution
-        if (rank == 0) {
-            const double log_s = log((double)S), log_p = log((double)psum);
-            double loss = 0;
-            for (int k = tid; k < pr.top; k += TEAM) {
-                const float d = (prob[k] - tmax) * inv_t, e = expf(d);
-                prob[k] = e;
-                if (idx[k] >= 0 && e > 0.f)
-                    loss += (double)e / (double)psum * (((double)d - log_p) - ((double)((to_float(z[idx[k]]) - m) * inv_t) - log_s));
-            }
-            loss = team.sum(loss);
-            if (tid == 0) {
-                const double t = pr.temperature;
-                pr.row_loss[row] = (float)(loss * t * t * (double)w * (double)pr.loss_factor);
-                pr.stats[row] = make_float2(m, S);
+                for (int e = 0; e < VEC; e++) o.v[e] = from_float<T>(v);
+                if (wide) {
+                    for (int i = v_first; i < sl.v1; i += TEAM) store_pack<T, VEC>(grad + sl.head + (long long)i * VEC, o);
+                    if (r_at >= 0) grad[r_at] = o.v[0];
+                } else {
+                    for (int j = from + tid; j < to; j += TEAM) grad[j] = o.v[0];
+                }
             }
         } else {
-            for (int k = tid; k < pr.top; k += TEAM) prob[k] = expf((prob[k] - tmax) * inv_t);
-        }
-    } else {
-        m = pr.stats[row].x;
-        S = pr.stats[row].y;
-    }
-    if (!GRAD) return;
-
-    const float a = up * pr.grad_factor * w * pr.temperature, inv_s = 1.f / S;
-    const int from = rank == 0 ? 0 : sl.head + sl.v0 * VEC, to = last ? pr.vocab : sl.head + sl.v1 * VEC;
-    const bool wide = ((uintptr_t)(grad + sl.head) & 15) == 0;
-    if (wide) {
-        if (rank == 0)
-            for (int j = tid; j < sl.head; j += TEAM) grad[j] = from_float<T>(ex2((to_float(z[j]) - m) * c) * inv_s * a);
-        if (last)
-            for (int j = sl.tail + tid; j < pr.vocab; j += TEAM) grad[j] = from_float<T>(ex2((to_float(z[j]) - m) * c) * inv_s * a);
-        const T *zv = z + sl.head;
-        T *gv = grad + sl.head;
-#pragma unroll 4
-        for (int i = sl.v0 + tid; i < sl.v1; i += TEAM) {
-            Pack<T, VEC> v = load_pack<T, VEC>(zv + (long long)i * VEC);
+            const float a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, inv_s = 1.f / sum, a_s = a * inv_s;
+            if (GRAD && streams) {
+                if (wide) {
+                    auto share = [&](const Pack<T, VEC> &v) {
+                        float f[VEC];
+                        Pack<T, VEC> o;
+                        unpack<VEC>(v, f);
 #pragma unroll
-            for (int e = 0; e < VEC; e++) v.v[e] = from_float<T>(ex2((to_float(v.v[e]) - m) * c) * inv_s * a);
-            store_pack<T, VEC>(gv + (long long)i * VEC, v);
-        }
-    } else {
-        for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2((to_float(z[j]) - m) * c) * inv_s * a);
-    }
-    team.sync();   // the entries' places are written a second time, after the pass above
-    for (int k = tid; k < pr.top; k += TEAM) {
-        const int j = idx[k];
-        if (j < from || j >= to) continue;
-        float p = 0.f;   // the entries of one index together, by the first of them
-        bool first = true;
-        for (int i = 0; i < pr.top; i++)
-            if (idx[i] == j) {
-                if (i < k) first = false;
-                p += prob[i];
+                        for (int e = 0; e < VEC; e++) f[e] = ex2(fmaf(f[e], c, -ref)) * a_s;
+                        pack<VEC>(o, f);
+                        return o;
+                    };
+                    T *out = grad + sl.head + (long long)v_first * VEC;
+#pragma unroll 4
+                    for (int h = 0; h < n_held - 1; h++) store_pack<T, VEC>(out + h * (TEAM * VEC), share(load_staged<T, VEC>(held + h * HOP)));
+                    if (n_held > 0 && v_first + (n_held - 1) * TEAM < sl.v1)
+                        store_pack<T, VEC>(out + (n_held - 1) * (TEAM * VEC), share(load_staged<T, VEC>(held + (n_held - 1) * HOP)));
+                    for (int i = v_far; i < sl.v1; i += TEAM) {
+                        Pack<T, VEC> v = load_pack<T, VEC>(zv + (long long)i * VEC);
+                        if (flat) {
+                            float f[VEC];
+                            unpack<VEC>(v, f);
+#pragma unroll
+                            for (int e = 0; e < VEC; e++) f[e] = seen(f[e]);
+                            pack<VEC>(v, f);
+                        }
+                        store_pack<T, VEC>(grad + sl.head + (long long)i * VEC, share(v));
+                    }
+                    if (r_at >= 0) grad[r_at] = from_float<T>(ex2(fmaf(r_value, c, -ref)) * a_s);
+                } else {   // the rows of the gradient lie otherwise in memory than those of the logits
+                    for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
+                }
             }
-        if (first) grad[j] = from_float<T>((ex2((to_float(z[j]) - m) * c) * inv_s - p * inv_psum) * a);
+            if (STATS && scribe && rank == 0) {
+                const double log_s = log((double)sum), log_p = log((double)psum);
+                double loss = 0;
+                for (int k = lane; k < pr.top; k += 32)
+                    if (en.idx[k] >= 0 && en.prob[k] > 0.f)
+                        loss += (double)en.prob[k] * (((double)en.diff[k] - log_p) - (((double)seen(en.own[k]) * (double)c - (double)ref) * 0.6931471805599453 - log_s));
+                loss = warp_sum(loss) / (double)psum;
+                if (lane == 0) {
+                    const double t = pr.temperature;
+                    pr.row_loss[row] = (float)(loss * t * t * (double)w * (double)pr.loss_factor);
+                    pr.stats[row] = make_float2(m, sum);
+                }
+            }
+            if (GRAD) {
+                team_sync();   // the entries' places are written a second time, after the pass above
+                for (int k = tid; k < pr.top; k += TEAM == 32 ? 32 : TEAM + 32)
+                    if (en.merged[k] >= 0.f) grad[en.idx[k]] = from_float<T>((ex2(fmaf(seen(en.own[k]), c, -ref)) * inv_s - en.merged[k]) * a);
+            }
+        }
+        if (row + teams < pr.rows) team_sync();   // before the next row's entries
     }
 }
 
@@ -297,14 +445,24 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const float *row_loss
 }
 
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER> int launch_team(const DistillParams &p, int ranks, cudaStream_t s) {
-    const int threads = TEAM == 32 ? 256 : TEAM;
-    const long long grid = TEAM == 32 ? (p.rows + 7) / 8 : p.rows * ranks;
-    if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows", p.rows);
-    const size_t smem = (size_t)(TEAM == 32 ? 8 : 1) * p.top * 8;
+    constexpr int threads = team_threads(TEAM);
+    long long grid = TEAM == 32 ? (p.rows + 3) / 4 : p.rows;
+    // a pass that may have nothing to do is not worth a CTA for every row: as many as are resident, walking over the rows
+    const long long resident = (long long)sm_count() * team_blocks(TEAM) / ranks;
+    if ((p.skip_one || grid * ranks > 0x7fffffffLL) && grid > resident) grid = resident;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)(grid * ranks));
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    const long long per_cta = ((long long)p.vocab * (long long)sizeof(T) / 16 + ranks - 1) / ranks;   // vectors of a CTA's slice at most
+    // whole warps of vectors: the lanes past a slice have a place too
+    const int team_bytes = entry_room(p.top) + (int)(per_cta < TEAM * DISTILL_HOLD ? (per_cta + 31) / 32 * 32 : TEAM * DISTILL_HOLD) * 16;
+    cfg.dynamicSmemBytes = (size_t)(TEAM == 32 ? 4 : 1) * team_bytes;
+    static PerDeviceOnce once;
+    int rc = per_device_once(once, []() -> int {
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, DISTILL_SMEM));
+        return GEO_SC_OK;
+    });
+    if (rc) return rc;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -312,15 +470,19 @@ template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER> int launch_
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CLUSTER ? 1 : 0;
-    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, p));
+    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, p, team_bytes));
     return GEO_SC_OK;
 }
 
 template <typename T, bool STATS, bool GRAD> int launch_distill(const DistillParams &p, cudaStream_t s) {
-    if (p.vocab <= DISTILL_WARP_VOCAB) return launch_team<T, 32, STATS, GRAD, false>(p, 1, s);
-    int ranks = 1;
-    while (ranks < 8 && p.rows * ranks * 2 <= sm_count() && p.vocab / (ranks * 2) >= 2048) ranks *= 2;
-    return ranks > 1 ? launch_team<T, 512, STATS, GRAD, true>(p, ranks, s) : launch_team<T, 512, STATS, GRAD, false>(p, 1, s);
+    // The smallest team that holds a row; twice the team, up to eight times, while that still leaves every SM one.
+    const long long vectors = (long long)p.vocab * sizeof(T) / 16;
+    int team = 32;
+    while (team < 2048 && (vectors > (long long)team * DISTILL_HOLD || (p.rows * team < 256LL * sm_count() && vectors > 2 * team))) team *= 2;
+    if (team == 32) return launch_team<T, 32, STATS, GRAD, false>(p, 1, s);
+    if (team <= 128) return launch_team<T, 128, STATS, GRAD, false>(p, 1, s);
+    if (team == 256) return launch_team<T, 256, STATS, GRAD, false>(p, 1, s);
+    return launch_team<T, 256, STATS, GRAD, true>(p, team / 256, s);
 }
 
 template <bool STATS, bool GRAD> int launch_typed(const DistillParams &p, int dtype, cudaStream_t s) {

@@ -92,20 +92,6 @@ template <typename T, int VEC> __device__ __forceinline__ void add_pack(Pack<T, 
     pack<VEC>(v, a);
 }
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {   // 16 bytes, zeros past `bytes`
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
-
-template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_staged(uint32_t at) {   // 16 bytes of shared memory
-    Pack<T, VEC> v;
-    int4 &r = *reinterpret_cast<int4 *>(&v);
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
-    return v;
-}
-
 // Statistics of a row, joined over its tpr threads (one or more warps of a CTA; part_* have room for two turns).
 struct RowStats {
     float ss;     // in the row's first warp

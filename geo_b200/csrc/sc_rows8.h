@@ -85,6 +85,29 @@ template <int N> __device__ __forceinline__ void pack(Pack<__half, N> &v, const 
         for (int e = 0; e < N / 2; e++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(f[2 * e + 1]), "f"(f[2 * e]));
     }
 }
+// Largest value of a pack (NaN passed over); two 16-bit values per instruction.
+template <int N> __device__ __forceinline__ float pack_max(const Pack<float, N> &v) {
+    float m = v.v[0];
+#pragma unroll
+    for (int e = 1; e < N; e++) m = fmaxf(m, v.v[e]);
+    return m;
+}
+template <int N> __device__ __forceinline__ float pack_max(const Pack<__nv_bfloat16, N> &v) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+    uint32_t m = w[0];
+#pragma unroll
+    for (int e = 1; e < N / 2; e++) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[e]));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+template <int N> __device__ __forceinline__ float pack_max(const Pack<__half, N> &v) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+    uint32_t m = w[0];
+#pragma unroll
+    for (int e = 1; e < N / 2; e++) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[e]));
+    float a, b;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}\n" : "=f"(a), "=f"(b) : "r"(m));
+    return fmaxf(a, b);
+}
 // Four signed bytes as floats: a byte b + 128 in the low mantissa of 2^23 is the float 2^23 + 128 + b, exactly.
 __device__ __forceinline__ void unpack_bytes(uint32_t w, float *f) {
     w ^= 0x80808080u;
@@ -102,10 +125,27 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+__device__ __forceinline__ float warp_max(float v) {   // NaN passed over
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {   // 16 bytes, zeros past `bytes`
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_staged(uint32_t at) {   // 16 bytes of shared memory
+    Pack<T, VEC> v;
+    int4 &r = *reinterpret_cast<int4 *>(&v);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
     return v;
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_staged(uint32_t at, const Pack<T, VEC> &v) {
+    const int4 &r = *reinterpret_cast<const int4 *>(&v);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 
 inline bool dtype_known(int dtype) { return dtype == GEO_SC_DTYPE_F32 || dtype == GEO_SC_DTYPE_BF16 || dtype == GEO_SC_DTYPE_F16; }

@@ -123,6 +123,27 @@ def test_masked_logits(cuda_device, dtype, vocab):
     assert loss[[0, 1, 2, 4]].isfinite().all() and grad[[0, 1, 2, 4]].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [41, 3000, 90001])
+def test_rows_at_the_ends_of_the_type(cuda_device, dtype, vocab):
+    """Rows masked by the type's lowest value throughout, or in part by -inf, and rows around the largest value: whatever
+    the temperature, logits that are equal have equal probabilities and the others none."""
+    logits, indices, teacher = make(4, vocab, 5, dtype, 3, cuda_device)
+    with torch.no_grad():
+        low = torch.finfo(dtype).min
+        logits[0] = low
+        logits[1] = -math.inf
+        logits[1, : vocab // 3] = low
+        indices[1] = torch.arange(5, device=cuda_device)
+        logits[2] = 0
+        logits[2, 3] = -low
+        logits[2, vocab - 2] = -low
+        indices[2], teacher[2, 1:] = 3, -math.inf
+    for T in (0.5, 1.0, 3.0):
+        check(logits, indices, teacher, T)
+        check(logits, indices, teacher, T, reduction="batchmean", up=torch.tensor(3.0, device=cuda_device))
+
+
 @pytest.mark.parametrize("vocab", [30, 2500])
 def test_bad_entries_poison_their_row_only(cuda_device, vocab):
     from geo_b200 import functional as F
