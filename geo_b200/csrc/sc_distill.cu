@@ -26,6 +26,8 @@
 // while the logits are on their way, and the loss while the gradient is written.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "sc_rows8.h"
 
 namespace geo {
@@ -34,7 +36,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int DISTILL_MAX_TOP = 512;
-constexpr int DISTILL_HOLD = 16;  // 16-byte vectors of a row that a thread holds
 constexpr float NEG_INF = -INFINITY;
 constexpr float FAR = 1073741824.f;   // 2^30
 
@@ -88,7 +89,9 @@ __device__ __forceinline__ float base_of(float r) { return r < -FAR ? 0.f : r; }
 __device__ __forceinline__ float moved(float sum, float from, float to) { return from < -FAR ? sum : sum * ex2(from - to); }
 
 constexpr int team_threads(int team) { return team == 32 ? 128 : team + 32; }   // four warps with a row each; or a team and the entries' warp
-constexpr int team_blocks(int team) { return team == 32 ? 8 : 896 / team; }         // that registers are left for, of an SM
+constexpr int team_blocks(int team, bool grad) { return team == 32 ? 8 : (grad ? 896 : 1280) / team; }         // that registers are left for, of an SM
+// 16-byte vectors of a row that a thread holds: for the gradient, or on their way only
+__host__ __device__ constexpr int held_vectors(bool grad) { return grad ? 16 : 8; }
 constexpr int DISTILL_SMEM = 200 * 1024;   // of an SM's 227 KB
 // a team's shared memory: 20 bytes per entry, the table that finds entries of the same index, then the team's vectors
 __host__ __device__ inline int table_slots(int top) {
@@ -171,8 +174,9 @@ __device__ __forceinline__ int take_entries(const DistillParams &pr, const Entri
 }
 
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER>
-__global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill_kernel(DistillParams pr, int team_bytes) {
+__global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) distill_kernel(DistillParams pr, int team_bytes) {
     constexpr int VEC = 16 / sizeof(T), WARPS = TEAM / 32, HOP = TEAM * 16;   // bytes between a thread's vectors
+    constexpr int GROUP = held_vectors(GRAD) / 4;
     extern __shared__ __align__(16) unsigned char distill_smem[];
     __shared__ float2 part[8];
     __shared__ float2 pair;   // this CTA's (largest logit, sum), read by the other CTAs of the cluster
@@ -217,28 +221,56 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
         const float w = pr.weight ? pr.weight[row] : 1.f;
         const int from = rank == 0 ? 0 : sl.head + sl.v0 * VEC, to = last ? pr.vocab : sl.head + sl.v1 * VEC;
 
-        // The same number of vectors for every lane of a warp; those past the slice are -inf.  From v_far on: read again.
-        int n_held = 0;
-        const int v_first = sl.v0 + tid, v_far = v_first + DISTILL_HOLD * TEAM;
+        // A thread's vectors: four groups of GROUP in shared memory, asked for at once.  Where a slice is longer, the next
+        // group takes the place of the one that has been read, and a second pass asks for them all again.  The lanes of a
+        // warp have the same number of vectors; those past the slice are -inf.
+        const int v_first = sl.v0 + tid;
+        const int ahead = sl.v1 - (sl.v0 + warp * 32);   // vectors from the warp's first on
+        const int count = streams ? max(0, ahead + TEAM - 1) / TEAM : 0, groups = (count + GROUP - 1) / GROUP;
+        const int whole = ahead >= 32 ? ((ahead - 32) / TEAM + 1) / GROUP : 0;   // groups that every lane has all of
+        auto fill = [&](int g) {
+            const T *src = zv + (long long)(v_first + g * (GROUP * TEAM)) * VEC;
+            const uint32_t dst = held + (g & 3) * (GROUP * HOP);
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int h = g * GROUP + i;
+                if (v_first + h * TEAM < sl.v1) {
+                    copy_async(dst + i * HOP, src + i * (TEAM * VEC), 16);
+                } else if (h < count) {
+                    Pack<T, VEC> none;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) none.v[e] = from_float<T>(NEG_INF);
+                    store_staged<T, VEC>(dst + i * HOP, none);
+                }
+            }
+            copy_commit();
+        };
+        auto fill_all = [&]() {
+            for (int g = 0; g < 4; g++) fill(g);
+        };
+        // f(vector, its place in shared memory) for every vector, when it has arrived; `resident`: all of them have, and stay
+        auto each = [&](bool resident, auto f) {
+            for (int g = 0; g < groups; g++) {
+                if (!resident) copy_wait<3>();
+                const uint32_t at = held + (g & 3) * (GROUP * HOP);
+                if (g < whole) {
+#pragma unroll
+                    for (int i = 0; i < GROUP; i++) f(g * GROUP + i, at + i * HOP, std::true_type());
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < GROUP && g * GROUP + i < count; i++) f(g * GROUP + i, at + i * HOP, std::false_type());
+                }
+                if (!resident) fill(g + 4);
+            }
+        };
         // the values before the first and after the last vector, one per thread
         int r_at = -1;
         float r_value = 0.f;
         if (streams) {
-            n_held = min(max(0, sl.v1 - (sl.v0 + warp * 32) + TEAM - 1) / TEAM, DISTILL_HOLD);
-            const T *src = zv + (long long)v_first * VEC;
-            uint32_t dst = held;
-            for (int h = 0; h < n_held; h++, src += TEAM * VEC, dst += HOP)
-                if (v_first + h * TEAM < sl.v1) copy_async(dst, src, 16);
-            if (n_held > 0 && v_first + (n_held - 1) * TEAM >= sl.v1) {
-                Pack<T, VEC> none;
-#pragma unroll
-                for (int e = 0; e < VEC; e++) none.v[e] = from_float<T>(NEG_INF);
-                store_staged<T, VEC>(held + (n_held - 1) * HOP, none);
-            }
+            fill_all();
             const int heads = rank == 0 ? sl.head : 0, ragged = heads + (last ? pr.vocab - sl.tail : 0);
             r_at = tid < heads ? tid : tid < ragged ? sl.tail + tid - heads : -1;
             if (r_at >= 0) r_value = to_float(z[r_at]);
-            copy_commit();
         }
         int state = 0;
         float psum = 1.f;
@@ -250,33 +282,32 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
             }
             __syncwarp();
         }
-        if (streams) copy_wait<0>();
 
         float m = 0.f, sum = 0.f;
         bool flat = false;   // m c out of range: a logit is either m or nothing
         auto seen = [&](float v) { return !flat ? v : v == m ? 0.f : NEG_INF; };
-        auto flatten = [&]() {
-            flat = true;
-            for (int h = 0; h < n_held; h++) {
-                float f[VEC];
-                Pack<T, VEC> v = load_staged<T, VEC>(held + h * HOP);
-                unpack<VEC>(v, f);
-#pragma unroll
-                for (int e = 0; e < VEC; e++) f[e] = seen(f[e]);
-                pack<VEC>(v, f);
-                store_staged<T, VEC>(held + h * HOP, v);
-            }
-            r_value = seen(r_value);
-        };
         auto out_of_range = [&]() { return fabsf(m) <= 3.402823466e38f && !(fabsf(scaled(m)) <= FAR); };
         // Largest logit and sum of the warp.  A thread's reference is the first largest value that it meets, and moves only
         // for one that is 2^32 times as probable (some lane would move it at nearly every vector otherwise); sums stay far
         // below 2^127.
-        auto warp_stats = [&](float &most, float &total) {
-            float top = r_at >= 0 ? r_value : NEG_INF;
-            if (n_held > 0) top = fmaxf(top, pack_max<VEC>(load_staged<T, VEC>(held)));
-            float ref = scaled(top), base = base_of(ref), s0 = r_at >= 0 ? ex2(fmaf(r_value, c, -base)) : 0.f, s1 = 0.f;
-            auto add = [&](const float (&f)[VEC], float large) {
+        auto warp_stats = [&](auto is_flat, float &most, float &total) {
+            constexpr bool FLAT = decltype(is_flat)::value;
+            float top = r_at >= 0 ? seen(r_value) : NEG_INF, ref = scaled(top), base = base_of(ref), s1 = 0.f;
+            float s0 = r_at >= 0 ? ex2(fmaf(top, c, -base)) : 0.f;
+            each(FLAT && groups <= 4, [&](int, uint32_t at, auto) {
+                const Pack<T, VEC> v = load_staged<T, VEC>(at);
+                float f[VEC], large;
+                unpack<VEC>(v, f);
+                if (FLAT) {
+                    large = NEG_INF;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        f[e] = seen(f[e]);
+                        large = fmaxf(large, f[e]);
+                    }
+                } else {
+                    large = pack_max<VEC>(v);
+                }
                 top = fmaxf(top, large);
                 if (scaled(large) > ref + 32.f) {
                     const float to_ref = scaled(large);
@@ -290,24 +321,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
                     s0 += ex2(fmaf(f[e], c, -base));
                     s1 += ex2(fmaf(f[e + 1], c, -base));
                 }
-            };
-#pragma unroll 4
-            for (int h = 0; h < n_held; h++) {
-                const Pack<T, VEC> v = load_staged<T, VEC>(held + h * HOP);
-                float f[VEC];
-                unpack<VEC>(v, f);
-                add(f, pack_max<VEC>(v));
-            }
-            for (int i = v_far; i < sl.v1; i += TEAM) {
-                float f[VEC], large = NEG_INF;
-                unpack<VEC>(load_pack<T, VEC>(zv + (long long)i * VEC), f);
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    f[e] = seen(f[e]);
-                    large = fmaxf(large, f[e]);
-                }
-                add(f, large);
-            }
+            });
             most = warp_max(top);
             total = warp_sum(moved(s0 + s1, ref, scaled(most)));
         };
@@ -315,7 +329,10 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
         if (STATS) {
             for (;;) {
                 float most = NEG_INF;
-                if (streams) warp_stats(most, sum);
+                if (streams) {
+                    if (flat) warp_stats(std::true_type(), most, sum);
+                    else warp_stats(std::false_type(), most, sum);
+                }
                 if (TEAM > 32) {
                     if (streams && lane == 0) part[warp] = make_float2(most, sum);
                     __syncthreads();
@@ -335,8 +352,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
                 if (flat) break;
                 m = most;
                 if (!out_of_range()) break;
-                if (streams) flatten();
                 flat = true;
+                if (groups > 4) fill_all();
                 team_sync();   // before the next partials
             }
             if (m == NEG_INF) sum = __int_as_float(0x7fc00000);   // no logit above -inf: no distribution
@@ -344,10 +361,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
             team_sync();
             m = pr.stats[row].x;
             sum = pr.stats[row].y;
-            if (out_of_range()) {
-                if (streams) flatten();
-                flat = true;
-            }
+            flat = out_of_range();
         }
         if (TEAM > 32) {
             state = row_state;
@@ -377,32 +391,23 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
             const float a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, inv_s = 1.f / sum, a_s = a * inv_s;
             if (GRAD && streams) {
                 if (wide) {
-                    auto share = [&](const Pack<T, VEC> &v) {
-                        float f[VEC];
-                        Pack<T, VEC> o;
-                        unpack<VEC>(v, f);
-#pragma unroll
-                        for (int e = 0; e < VEC; e++) f[e] = ex2(fmaf(f[e], c, -ref)) * a_s;
-                        pack<VEC>(o, f);
-                        return o;
-                    };
+                    const bool resident = STATS && groups <= 4;
+                    if (STATS && !resident) fill_all();
                     T *out = grad + sl.head + (long long)v_first * VEC;
-#pragma unroll 4
-                    for (int h = 0; h < n_held - 1; h++) store_pack<T, VEC>(out + h * (TEAM * VEC), share(load_staged<T, VEC>(held + h * HOP)));
-                    if (n_held > 0 && v_first + (n_held - 1) * TEAM < sl.v1)
-                        store_pack<T, VEC>(out + (n_held - 1) * (TEAM * VEC), share(load_staged<T, VEC>(held + (n_held - 1) * HOP)));
-                    for (int i = v_far; i < sl.v1; i += TEAM) {
-                        Pack<T, VEC> v = load_pack<T, VEC>(zv + (long long)i * VEC);
-                        if (flat) {
+                    auto give = [&](auto is_flat) {
+                        each(resident, [&](int h, uint32_t at, auto all_lanes) {
                             float f[VEC];
-                            unpack<VEC>(v, f);
+                            unpack<VEC>(load_staged<T, VEC>(at), f);
 #pragma unroll
-                            for (int e = 0; e < VEC; e++) f[e] = seen(f[e]);
-                            pack<VEC>(v, f);
-                        }
-                        store_pack<T, VEC>(grad + sl.head + (long long)i * VEC, share(v));
-                    }
-                    if (r_at >= 0) grad[r_at] = from_float<T>(ex2(fmaf(r_value, c, -ref)) * a_s);
+                            for (int e = 0; e < VEC; e++) f[e] = ex2(fmaf(decltype(is_flat)::value ? seen(f[e]) : f[e], c, -ref)) * a_s;
+                            Pack<T, VEC> o;
+                            pack<VEC>(o, f);
+                            if (decltype(all_lanes)::value || v_first + h * TEAM < sl.v1) store_pack<T, VEC>(out + (long long)h * (TEAM * VEC), o);
+                        });
+                    };
+                    if (flat) give(std::true_type());
+                    else give(std::false_type());
+                    if (r_at >= 0) grad[r_at] = from_float<T>(ex2(fmaf(seen(r_value), c, -ref)) * a_s);
                 } else {   // the rows of the gradient lie otherwise in memory than those of the logits
                     for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
                 }
@@ -426,6 +431,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM)) distill
                     if (en.merged[k] >= 0.f) grad[en.idx[k]] = from_float<T>((ex2(fmaf(seen(en.own[k]), c, -ref)) * inv_s - en.merged[k]) * a);
             }
         }
+        copy_wait<0>();
         if (row + teams < pr.rows) team_sync();   // before the next row's entries
     }
 }
@@ -448,14 +454,14 @@ template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER> int launch_
     constexpr int threads = team_threads(TEAM);
     long long grid = TEAM == 32 ? (p.rows + 3) / 4 : p.rows;
     // a pass that may have nothing to do is not worth a CTA for every row: as many as are resident, walking over the rows
-    const long long resident = (long long)sm_count() * team_blocks(TEAM) / ranks;
+    const long long resident = (long long)sm_count() * team_blocks(TEAM, GRAD) / ranks;
     if ((p.skip_one || grid * ranks > 0x7fffffffLL) && grid > resident) grid = resident;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(grid * ranks));
     cfg.blockDim = dim3(threads);
     const long long per_cta = ((long long)p.vocab * (long long)sizeof(T) / 16 + ranks - 1) / ranks;   // vectors of a CTA's slice at most
     // whole warps of vectors: the lanes past a slice have a place too
-    const int team_bytes = entry_room(p.top) + (int)(per_cta < TEAM * DISTILL_HOLD ? (per_cta + 31) / 32 * 32 : TEAM * DISTILL_HOLD) * 16;
+    const int team_bytes = entry_room(p.top) + (int)(per_cta < TEAM * held_vectors(GRAD) ? (per_cta + 31) / 32 * 32 : TEAM * held_vectors(GRAD)) * 16;
     cfg.dynamicSmemBytes = (size_t)(TEAM == 32 ? 4 : 1) * team_bytes;
     static PerDeviceOnce once;
     int rc = per_device_once(once, []() -> int {
@@ -475,10 +481,11 @@ template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER> int launch_
 }
 
 template <typename T, bool STATS, bool GRAD> int launch_distill(const DistillParams &p, cudaStream_t s) {
-    // The smallest team that holds a row; twice the team, up to eight times, while that still leaves every SM one.
+    // The smallest team that holds a row, or, for the loss alone, gives every thread some vectors; twice the team, up to
+    // eight times, while that still leaves every SM one.
     const long long vectors = (long long)p.vocab * sizeof(T) / 16;
     int team = 32;
-    while (team < 2048 && (vectors > (long long)team * DISTILL_HOLD || (p.rows * team < 256LL * sm_count() && vectors > 2 * team))) team *= 2;
+    while (team < 2048 && ((GRAD || team < 256 ? vectors > (long long)team * 16 : false) || (p.rows * team < 256LL * sm_count() && vectors > 2 * team))) team *= 2;
     if (team == 32) return launch_team<T, 32, STATS, GRAD, false>(p, 1, s);
     if (team <= 128) return launch_team<T, 128, STATS, GRAD, false>(p, 1, s);
     if (team == 256) return launch_team<T, 256, STATS, GRAD, false>(p, 1, s);
