@@ -49,16 +49,37 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[j][i] = 0;
     }
-#pragma unroll 2
-    for (int kc = warp * 64; kc < p.k; kc += MMA_WARPS * 64) {
-        const int at = kc + t * 16;
-        const uint4 a = load16(wa, at, p.k), b = load16(wb, at, p.k);
+    auto step = [&](const uint4 &a, const uint4 &b, const uint4 (&x)[NT]) {
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            const uint4 x = load16(xr[j], at, p.k);
-            mma_s8(acc[j], a.x, b.x, a.y, b.y, x.x, x.y);
-            mma_s8(acc[j], a.z, b.z, a.w, b.w, x.z, x.w);
+            mma_s8(acc[j], a.x, b.x, a.y, b.y, x[j].x, x[j].y);
+            mma_s8(acc[j], a.z, b.z, a.w, b.w, x[j].z, x[j].w);
         }
+    };
+    // UNROLL chunks of 64 bytes of k per warp at a time, their weights all asked for before the first is used
+    constexpr int UNROLL = NT == 1 ? 4 : 2, TURN = MMA_WARPS * 64;
+    int kc = warp * 64;
+    for (; kc + (UNROLL - 1) * TURN + 64 <= p.k; kc += UNROLL * TURN) {
+        uint4 a[UNROLL], b[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            a[u] = __ldg((const uint4 *)(wa + kc + u * TURN + t * 16));
+            b[u] = __ldg((const uint4 *)(wb + kc + u * TURN + t * 16));
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            uint4 x[NT];
+#pragma unroll
+            for (int j = 0; j < NT; j++) x[j] = __ldg((const uint4 *)(xr[j] + kc + u * TURN + t * 16));
+            step(a[u], b[u], x);
+        }
+    }
+    for (; kc < p.k; kc += TURN) {
+        const uint4 a = load16(wa, kc + t * 16, p.k), b = load16(wb, kc + t * 16, p.k);
+        uint4 x[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) x[j] = load16(xr[j], kc + t * 16, p.k);
+        step(a, b, x);
     }
 #pragma unroll
     for (int j = 0; j < NT; j++) {
@@ -110,7 +131,7 @@ extern "C" int geo_sc_linear_int8(int m, int n, int k, const int8_t *x, long lon
         return fail(GEO_SC_ERR_UNSUPPORTED, "rows of x and w have to start on 16-byte boundaries");
     LinearParams p{x, w, x_scale, w_scale, bias, out, x_stride, w_stride, out_stride, m, n, k};
     cudaStream_t s = (cudaStream_t)stream;
-    if (m > 32) return launch_linear_int8_tc(p, dtype, s);
+    if (m > 8) return launch_linear_int8_tc(p, dtype, s);
     if (dtype == GEO_SC_DTYPE_F32) return launch_mma<float>(p, s);
     if (dtype == GEO_SC_DTYPE_BF16) return launch_mma<__nv_bfloat16>(p, s);
     return launch_mma<__half>(p, s);

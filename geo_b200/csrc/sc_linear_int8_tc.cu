@@ -8,6 +8,13 @@
 // (cta_group::2): each of the pair loads its 128 channels and half of the tokens, the even CTA issues the
 // instructions for both, and each keeps the accumulators of its own channels.
 //
+// Where there are fewer tiles than SMs a cluster of 2, 4 or 8 CTAs shares a tile: each sums a part of k, leaves its
+// integers in its shared memory, and takes a part of the columns over the cluster's shared memory (integers: the order
+// of the additions does not matter).
+//
+// What bounds it: large products the matrix instructions; products of few tokens the bytes that an SM can pull in, about
+// 64 a clock, which is why small tiles on many SMs win over large tiles on few (choose_tile).
+//
 // Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
 // out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the
 // CTA stops waiting, lets its own copies and instructions in flight finish (again with a bound) and leaves.
@@ -124,40 +131,56 @@ template <int CTAS> __device__ __forceinline__ void tmem_free(uint32_t base, uin
     if (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+#define LT_REGS32(x) x(0), x(1), x(2), x(3), x(4), x(5), x(6), x(7), x(8), x(9), x(10), x(11), x(12), x(13), x(14), x(15), x(16), x(17), x(18), x(19), x(20), x(21), x(22), x(23), x(24), x(25), x(26), x(27), x(28), x(29), x(30), x(31)
+#define LT_OUT(i) "=r"(r[i])
+#define LT_INOUT(i) "+r"(r[i])
+#define LT_OUT16(x) x(0), x(1), x(2), x(3), x(4), x(5), x(6), x(7), x(8), x(9), x(10), x(11), x(12), x(13), x(14), x(15)
+// N columns of the warp's 32 lanes; the registers may be read after tmem_ld_wait (they pass through it, so that nothing
+// that reads them moves up).
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+                 : LT_REGS32(LT_OUT)
                  : "r"(taddr)
                  : "memory");
 }
-// The registers of the load above may be read from here on (they pass through, so that nothing that reads them moves up).
-__device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                 : LT_OUT16(LT_OUT)
+                 : "r"(taddr)
                  : "memory");
 }
-template <int CTAS> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the pair
-    if (CTAS == 1) __syncthreads();
+__device__ __forceinline__ void tmem_ld_wait(int (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS32(LT_INOUT) : : "memory"); }
+__device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_OUT16(LT_INOUT) : : "memory"); }
+__device__ __forceinline__ int load_remote(uint32_t addr, int cta) {   // the same place in another CTA of the cluster
+    uint32_t r;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(cta));
+    asm volatile("ld.shared::cluster.b32 %0, [%1];\n" : "=r"(v) : "r"(r) : "memory");
+    return v;
+}
+template <bool CLUSTER> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the cluster
+    if (!CLUSTER) __syncthreads();
     else asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
 
-template <typename T, int CTAS, int BN>
+// SPLIT: a cluster shares one tile and splits k; else CTAs (or pairs of them) walk over the tiles.
+template <typename T, int CTAS, int BN, bool SPLIT>
 __global__ void __launch_bounds__(LT_THREADS, 1)
-linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearParams pr, int ntiles_n, int ntiles) {
+linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearParams pr, int ntiles_n, int ntiles, int splits) {
     using Tile = LinearTile<CTAS, BN>;
-    constexpr int ST = Tile::STAGES;
+    constexpr int ST = Tile::STAGES, COLS = BN / 2;   // columns of an epilogue warp: two warps share a lane quarter
+    constexpr int CH = COLS < 32 ? COLS : 32;         // columns read out at a time
     extern __shared__ unsigned char lt_smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 5];   // full, empty, acc_full[2], acc_empty[2], drain
-    __shared__ __align__(16) float scales[LT_EPI_WARPS][16];
+    __shared__ __align__(16) float scales[LT_EPI_WARPS][COLS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const uint32_t tiles = (smem_u32(lt_smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1), worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);
+    const int part = SPLIT ? (int)blockIdx.x % splits : 0;
+    const int worker = SPLIT ? blockIdx.x / splits : blockIdx.x / CTAS, workers = SPLIT ? ntiles : gridDim.x / CTAS;
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
     auto empty_bar = [&](int s) { return bar0 + 8u * (ST + s); };
@@ -176,10 +199,11 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     if (warp == 1) tmem_alloc<CTAS>(smem_u32(&tmem_slot), Tile::TMEM_COLS);
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    tile_sync<CTAS>();
+    tile_sync<CTAS == 2>();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
-    const int nkb = (pr.k + LT_KB - 1) / LT_KB;
+    const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
+    const int kb0 = SPLIT ? (int)((long long)all_kb * part / splits) : 0, kb1 = SPLIT ? (int)((long long)all_kb * (part + 1) / splits) : all_kb;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -187,7 +211,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             bool ok = true;
             for (int t = worker; t < ntiles && ok; t += workers) {
                 const int n0 = (t % ntiles_n) * 128 * CTAS + rank * 128, m0 = (t / ntiles_n) * BN + rank * Tile::X_ROWS;
-                for (int kb = 0; kb < nkb; kb++, it++) {
+                for (int kb = kb0; kb < kb1; kb++, it++) {
                     const int s = it % ST;
                     if (!(ok = mbar_wait(empty_bar(s), ((it / ST) & 1) ^ 1, abort))) break;
                     if (rank == 0) mbar_expect_tx(full_bar(s), (uint32_t)(CTAS * Tile::STAGE));
@@ -207,7 +231,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             for (int t = worker; t < ntiles && ok; t += workers, n++) {
                 const int a = n & 1;
                 if (!(ok = mbar_wait(acce_bar(a), ((n >> 1) & 1) ^ 1, abort))) break;
-                for (int kb = 0; kb < nkb; kb++, it++) {
+                for (int kb = kb0; kb < kb1; kb++, it++) {
                     const int s = it % ST;
                     if (!(ok = mbar_wait(full_bar(s), (it / ST) & 1, abort))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -215,7 +239,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     const uint64_t adesc = umma_desc(st), bdesc = umma_desc(st + 128 * LT_KB);
 #pragma unroll
                     for (int k = 0; k < LT_KB / 32; k++)   // 32 bytes further along k: + 2 in units of 16 bytes
-                        umma_i8<CTAS>(tmem_base + a * BN, adesc + 2 * k, bdesc + 2 * k, Tile::IDESC, (kb | k) != 0);
+                        umma_i8<CTAS>(tmem_base + a * BN, adesc + 2 * k, bdesc + 2 * k, Tile::IDESC, (kb - kb0) | k ? 1u : 0u);
                     umma_commit<CTAS>(empty_bar(s));
                 }
                 if (ok) umma_commit<CTAS>(accf_bar(a));
@@ -227,29 +251,43 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         }
     } else {
         const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
-        constexpr int COLS = BN / 2;   // columns of a warp: two warps share a lane quarter
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * COLS;
         int n = 0;
         for (int t = worker; t < ntiles; t += workers, n++) {
             const int a = n & 1;
             const int ch = (t % ntiles_n) * 128 * CTAS + rank * 128 + quarter * 32 + lane, m0 = (t / ntiles_n) * BN + half * COLS;
             const float ws = ch < pr.n ? pr.w_scale[ch] : 0.f, b = pr.bias && ch < pr.n ? pr.bias[ch] : 0.f;
+            if (!SPLIT) {   // the tile's token scales, while it is being summed
+                for (int c = lane; c < COLS; c += 32) scales[ew][c] = m0 + c < pr.m ? pr.x_scale[m0 + c] : 0.f;
+                __syncwarp();
+            }
             if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            T *out = (T *)pr.out + (long long)m0 * pr.out_stride + ch;
+            const bool whole = !SPLIT && ch - lane + 32 <= pr.n && m0 + COLS <= pr.m;
 #pragma unroll 1
-            for (int c = 0; c < COLS; c += 16) {
-                int v[16];
-                tmem_ld16(lane_addr + a * BN + c, v);
-                __syncwarp();
-                if (lane < 16) scales[ew][lane] = m0 + c + lane < pr.m ? pr.x_scale[m0 + c + lane] : 0.f;
-                __syncwarp();
+            for (int c = 0; c < COLS; c += CH) {
+                int v[CH];
+                tmem_ld(lane_addr + a * BN + c, v);
                 tmem_ld_wait(v);
-                T *out = (T *)pr.out + (long long)(m0 + c) * pr.out_stride + ch;
+                if constexpr (SPLIT) {   // columns of 128 lanes; the tiles' shared memory is free (every instruction has read it)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    float y = (float)v[j] * scales[ew][j] * ws;
-                    if (pr.bias) y += b;
-                    if (ch < pr.n && m0 + c + j < pr.m) out[j * pr.out_stride] = from_float<T>(y);
+                    for (int j = 0; j < CH; j++)
+                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(tiles + (uint32_t)((half * COLS + c + j) * 128 + quarter * 32 + lane) * 4u), "r"(v[j]) : "memory");
+                } else if (whole) {
+#pragma unroll
+                    for (int j = 0; j < CH; j++, out += pr.out_stride) {
+                        float y = (float)v[j] * scales[ew][c + j] * ws;
+                        if (pr.bias) y += b;
+                        *out = from_float<T>(y);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < CH; j++, out += pr.out_stride) {
+                        float y = (float)v[j] * scales[ew][c + j] * ws;
+                        if (pr.bias) y += b;
+                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>(y);
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -259,7 +297,25 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    tile_sync<CTAS>();   // nobody leaves while the other CTA of the pair may still reach its barriers
+    tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all sums are there
+    if (SPLIT) {
+        // this CTA's share of the columns: from every CTA of the cluster, 32 neighbouring channels of one token per warp
+        const int share = BN / splits, t = worker;
+        for (int i = warp; i < share * 4; i += LT_THREADS / 32) {
+            const int col = part * share + (i >> 2), l = (i & 3) * 32 + lane;
+            const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
+            int v[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) v[r] = r < splits ? load_remote(tiles + (uint32_t)(col * 128 + l) * 4u, r) : 0;
+            const int sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            if (ch < pr.n && m < pr.m) {
+                float y = (float)sum * pr.x_scale[m] * pr.w_scale[ch];
+                if (pr.bias) y += pr.bias[ch];
+                ((T *)pr.out)[(long long)m * pr.out_stride + ch] = from_float<T>(y);
+            }
+        }
+        tile_sync<true>();   // nobody leaves while its sums are read
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         tmem_free<CTAS>(tmem_base, Tile::TMEM_COLS);
@@ -291,7 +347,7 @@ int encode_rows(CUtensorMap *map, const int8_t *base, int k, int rows, long long
     return r == CUDA_SUCCESS ? GEO_SC_OK : fail(GEO_SC_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
 }
 
-template <typename T, int CTAS, int BN> int launch_tile(const LinearParams &p, cudaStream_t s) {
+template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const LinearParams &p, int splits, cudaStream_t s) {
     using Tile = LinearTile<CTAS, BN>;
     CUtensorMap map_w, map_x;
     int rc = encode_rows(&map_w, p.w, p.k, p.n, p.w_stride, 128);
@@ -299,35 +355,64 @@ template <typename T, int CTAS, int BN> int launch_tile(const LinearParams &p, c
     if (rc) return rc;
     static PerDeviceOnce once;
     rc = per_device_once(once, []() -> int {
-        GEO_CUDA_CHECK(cudaFuncSetAttribute(linear_int8_tc_kernel<T, CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::SMEM));
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(linear_int8_tc_kernel<T, CTAS, BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile::SMEM));
         return GEO_SC_OK;
     });
     if (rc) return rc;
     const int tn = (p.n + 128 * CTAS - 1) / (128 * CTAS);
     const long long tiles = (long long)tn * ((p.m + BN - 1) / BN);
     if (tiles > 0x3fffffff) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
-    const int workers = sm_count() / CTAS;
+    const int workers = SPLIT ? (int)tiles : (int)(tiles < sm_count() / CTAS ? tiles : sm_count() / CTAS), cluster = SPLIT ? splits : CTAS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((tiles < workers ? (int)tiles : workers) * CTAS));
+    cfg.gridDim = dim3((unsigned)(workers * cluster));
     cfg.blockDim = dim3(LT_THREADS);
     cfg.dynamicSmemBytes = Tile::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CTAS > 1 ? 1 : 0;
-    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_int8_tc_kernel<T, CTAS, BN>, map_w, map_x, p, tn, (int)tiles));
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_int8_tc_kernel<T, CTAS, BN, SPLIT>, map_w, map_x, p, tn, (int)tiles, splits));
     return GEO_SC_OK;
 }
 
+// The tile and the split of k with the least estimated time.  A CTA's stage (128 bytes of k) takes the clocks of its bytes
+// at 64 a clock or of its matrix instructions, whichever is more: 2 (128 + rows of x).  A turn over a tile costs about
+// 1000 clocks more, joining a split one about 3000.
+struct TileChoice { int pair, bn, splits; };
+TileChoice choose_tile(const LinearParams &p) {
+    const long long sms = sm_count(), kb = (p.k + LT_KB - 1) / LT_KB;
+    TileChoice best{0, 64, 1};
+    long long least = -1;
+    auto consider = [&](int pair, int bn, int splits) {
+        const long long ctas = pair ? 2 : 1, tiles = ((p.n + 128 * ctas - 1) / (128 * ctas)) * ((p.m + bn - 1) / bn);
+        if (splits > 1 && (tiles * splits > sms || kb < 2 * splits)) return;
+        const long long turns = (tiles * ctas * splits + sms - 1) / sms;
+        const long long cost = turns * ((kb + splits - 1) / splits * 2 * (128 + bn / ctas) + 1000) + (splits > 1 ? 3000 : 0);
+        if (least < 0 || cost < least) {
+            least = cost;
+            best = TileChoice{pair, bn, splits};
+        }
+    };
+    consider(1, 256, 1);
+    for (int bn = 128; bn >= 32; bn /= 2)
+        for (int splits = 1; splits <= 8; splits *= 2) consider(0, bn, splits);
+    return best;
+}
+
 template <typename T> int launch_tc(const LinearParams &p, cudaStream_t s) {
-    // the largest tile that still gives most SMs one
-    const long long tn = (p.n + 127) / 128, sms = sm_count();
-    if (p.m > 128 && tn * ((p.m + 255) / 256) >= sms) return launch_tile<T, 2, 256>(p, s);
-    if (p.m > 64 && tn * ((p.m + 127) / 128) >= sms) return launch_tile<T, 1, 128>(p, s);
-    return p.m <= 32 ? launch_tile<T, 1, 32>(p, s) : launch_tile<T, 1, 64>(p, s);
+    const TileChoice c = choose_tile(p);
+    if (c.pair) return launch_tile<T, 2, 256, false>(p, 1, s);
+    if (c.splits > 1) {
+        if (c.bn == 128) return launch_tile<T, 1, 128, true>(p, c.splits, s);
+        if (c.bn == 64) return launch_tile<T, 1, 64, true>(p, c.splits, s);
+        return launch_tile<T, 1, 32, true>(p, c.splits, s);
+    }
+    if (c.bn == 128) return launch_tile<T, 1, 128, false>(p, 1, s);
+    if (c.bn == 64) return launch_tile<T, 1, 64, false>(p, 1, s);
+    return launch_tile<T, 1, 32, false>(p, 1, s);
 }
 
 }  // namespace
