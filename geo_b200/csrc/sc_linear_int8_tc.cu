@@ -189,6 +189,10 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const uint32_t drain_bar = bar0 + 8u * (2 * ST + 4);
     volatile int *abort = &abort_flag;
 
+    if (threadIdx.x == 32 * 2) {   // the first copies would wait for these
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
+    }
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < ST; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
@@ -264,6 +268,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             T *out = (T *)pr.out + (long long)m0 * pr.out_stride + ch;
+            const bool paired = pr.out_stride % 2 == 0 && ((uintptr_t)pr.out & 3) == 0;
             const bool whole = !SPLIT && ch - lane + 32 <= pr.n && m0 + COLS <= pr.m;
 #pragma unroll 1
             for (int c = 0; c < COLS; c += CH) {
@@ -274,19 +279,24 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 #pragma unroll
                     for (int j = 0; j < CH; j++)
                         asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(tiles + (uint32_t)((half * COLS + c + j) * 128 + quarter * 32 + lane) * 4u), "r"(v[j]) : "memory");
+                } else if (whole && sizeof(T) == 2 && paired) {
+                    // two tokens at a time: the even lane of a pair of channels stores both of one token, the odd lane of the other
+#pragma unroll
+                    for (int j = 0; j < CH; j += 2, out += 2 * pr.out_stride) {
+                        float y0 = (float)v[j] * scales[ew][c + j] * ws + b, y1 = (float)v[j + 1] * scales[ew][c + j + 1] * ws + b;
+                        const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? y0 : y1, 1);
+                        Pack<T, 2> o;
+                        const float f[2] = {lane & 1 ? other : y0, lane & 1 ? y1 : other};
+                        pack<2>(o, f);
+                        store_pack<T, 2>(lane & 1 ? out + pr.out_stride - 1 : out, o);
+                    }
                 } else if (whole) {
 #pragma unroll
-                    for (int j = 0; j < CH; j++, out += pr.out_stride) {
-                        float y = (float)v[j] * scales[ew][c + j] * ws;
-                        if (pr.bias) y += b;
-                        *out = from_float<T>(y);
-                    }
+                    for (int j = 0; j < CH; j++, out += pr.out_stride) *out = from_float<T>((float)v[j] * scales[ew][c + j] * ws + b);
                 } else {
 #pragma unroll
                     for (int j = 0; j < CH; j++, out += pr.out_stride) {
-                        float y = (float)v[j] * scales[ew][c + j] * ws;
-                        if (pr.bias) y += b;
-                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>(y);
+                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>((float)v[j] * scales[ew][c + j] * ws + b);
                     }
                 }
             }
@@ -300,18 +310,29 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all sums are there
     if (SPLIT) {
         // this CTA's share of the columns: from every CTA of the cluster, 32 neighbouring channels of one token per warp
-        const int share = BN / splits, t = worker;
-        for (int i = warp; i < share * 4; i += LT_THREADS / 32) {
-            const int col = part * share + (i >> 2), l = (i & 3) * 32 + lane;
-            const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
-            int v[8];
+        const int share = BN / splits, units = share * 4, t = worker;
+        constexpr int AT_ONCE = 4;   // units of a warp whose loads are in flight together
+        for (int u = warp; u < units; u += AT_ONCE * (LT_THREADS / 32)) {
+            int v[AT_ONCE][8];
+            float xs[AT_ONCE], ws[AT_ONCE], b[AT_ONCE];
 #pragma unroll
-            for (int r = 0; r < 8; r++) v[r] = r < splits ? load_remote(tiles + (uint32_t)(col * 128 + l) * 4u, r) : 0;
-            const int sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-            if (ch < pr.n && m < pr.m) {
-                float y = (float)sum * pr.x_scale[m] * pr.w_scale[ch];
-                if (pr.bias) y += pr.bias[ch];
-                ((T *)pr.out)[(long long)m * pr.out_stride + ch] = from_float<T>(y);
+            for (int i = 0; i < AT_ONCE; i++) {
+                const int unit = u + i * (LT_THREADS / 32), col = part * share + (unit >> 2), l = (unit & 3) * 32 + lane;
+                const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
+                const bool in = unit < units && ch < pr.n && m < pr.m;
+#pragma unroll
+                for (int r = 0; r < 8; r++) v[i][r] = unit < units && r < splits ? load_remote(tiles + (uint32_t)(col * 128 + l) * 4u, r) : 0;
+                xs[i] = in ? pr.x_scale[m] : 0.f;
+                ws[i] = in ? pr.w_scale[ch] : 0.f;
+                b[i] = in && pr.bias ? pr.bias[ch] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; i++) {
+                const int unit = u + i * (LT_THREADS / 32), col = part * share + (unit >> 2), l = (unit & 3) * 32 + lane;
+                const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
+                const int sum = ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
+                if (unit < units && ch < pr.n && m < pr.m)
+                    ((T *)pr.out)[(long long)m * pr.out_stride + ch] = from_float<T>((float)sum * xs[i] * ws[i] + b[i]);
             }
         }
         tile_sync<true>();   // nobody leaves while its sums are read
