@@ -56,31 +56,36 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
             mma_s8(acc[j], a.z, b.z, a.w, b.w, x[j].z, x[j].w);
         }
     };
-    // UNROLL chunks of 64 bytes of k per warp at a time, their weights all asked for before the first is used
-    constexpr int UNROLL = NT == 1 ? 4 : 2, TURN = MMA_WARPS * 64;
-    int kc = warp * 64;
-    for (; kc + (UNROLL - 1) * TURN + 64 <= p.k; kc += UNROLL * TURN) {
+    // A warp's turn: 128 bytes (two chunks) of every row, whole lines; with few tokens two turns at a time, their weights
+    // all asked for before the first is used.
+    constexpr int UNROLL = NT == 1 ? 4 : 2, TURN = MMA_WARPS * 128;
+    auto chunk = [&](int u) { return (u >> 1) * TURN + (u & 1) * 64 + t * 16; };
+    int kc = warp * 128;
+    for (; kc + (UNROLL / 2 - 1) * TURN + 128 <= p.k; kc += UNROLL / 2 * TURN) {
         uint4 a[UNROLL], b[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            a[u] = __ldg((const uint4 *)(wa + kc + u * TURN + t * 16));
-            b[u] = __ldg((const uint4 *)(wb + kc + u * TURN + t * 16));
+            a[u] = __ldg((const uint4 *)(wa + kc + chunk(u)));
+            b[u] = __ldg((const uint4 *)(wb + kc + chunk(u)));
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             uint4 x[NT];
 #pragma unroll
-            for (int j = 0; j < NT; j++) x[j] = __ldg((const uint4 *)(xr[j] + kc + u * TURN + t * 16));
+            for (int j = 0; j < NT; j++) x[j] = __ldg((const uint4 *)(xr[j] + kc + chunk(u)));
             step(a[u], b[u], x);
         }
     }
-    for (; kc < p.k; kc += TURN) {
-        const uint4 a = load16(wa, kc + t * 16, p.k), b = load16(wb, kc + t * 16, p.k);
-        uint4 x[NT];
+    for (; kc < p.k; kc += TURN)
 #pragma unroll
-        for (int j = 0; j < NT; j++) x[j] = load16(xr[j], kc + t * 16, p.k);
-        step(a, b, x);
-    }
+        for (int u = 0; u < 2; u++) {
+            const int at = kc + chunk(u);
+            const uint4 a = load16(wa, at, p.k), b = load16(wb, at, p.k);
+            uint4 x[NT];
+#pragma unroll
+            for (int j = 0; j < NT; j++) x[j] = load16(xr[j], at, p.k);
+            step(a, b, x);
+        }
 #pragma unroll
     for (int j = 0; j < NT; j++) {
         sums[warp][j * 8 + t * 2][g] = acc[j][0];
@@ -131,7 +136,7 @@ extern "C" int geo_sc_linear_int8(int m, int n, int k, const int8_t *x, long lon
         return fail(GEO_SC_ERR_UNSUPPORTED, "rows of x and w have to start on 16-byte boundaries");
     LinearParams p{x, w, x_scale, w_scale, bias, out, x_stride, w_stride, out_stride, m, n, k};
     cudaStream_t s = (cudaStream_t)stream;
-    if (m > 8) return launch_linear_int8_tc(p, dtype, s);
+    if (m > 32) return launch_linear_int8_tc(p, dtype, s);
     if (dtype == GEO_SC_DTYPE_F32) return launch_mma<float>(p, s);
     if (dtype == GEO_SC_DTYPE_BF16) return launch_mma<__nv_bfloat16>(p, s);
     return launch_mma<__half>(p, s);

@@ -20,6 +20,7 @@
 // CTA stops waiting, lets its own copies and instructions in flight finish (again with a bound) and leaves.
 #include <cuda.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "sc_linear_int8.h"
@@ -152,11 +153,11 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_ld_wait(int (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS32(LT_INOUT) : : "memory"); }
 __device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_OUT16(LT_INOUT) : : "memory"); }
-__device__ __forceinline__ int load_remote(uint32_t addr, int cta) {   // the same place in another CTA of the cluster
+__device__ __forceinline__ int4 load_remote(uint32_t addr, int cta) {   // 16 bytes at the same place in another CTA of the cluster
     uint32_t r;
-    int v;
+    int4 v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(cta));
-    asm volatile("ld.shared::cluster.b32 %0, [%1];\n" : "=r"(v) : "r"(r) : "memory");
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(r) : "memory");
     return v;
 }
 template <bool CLUSTER> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the cluster
@@ -174,6 +175,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     extern __shared__ unsigned char lt_smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 5];   // full, empty, acc_full[2], acc_empty[2], drain
     __shared__ __align__(16) float scales[LT_EPI_WARPS][COLS];
+    __shared__ __align__(16) float split_x[SPLIT ? BN : 1], split_w[SPLIT ? 128 : 1], split_b[SPLIT ? 128 : 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const uint32_t tiles = (smem_u32(lt_smem_raw) + 1023u) & ~1023u;
@@ -207,7 +209,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
     const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
-    const int kb0 = SPLIT ? (int)((long long)all_kb * part / splits) : 0, kb1 = SPLIT ? (int)((long long)all_kb * (part + 1) / splits) : all_kb;
+    const int kb0 = SPLIT ? all_kb * part / splits : 0, kb1 = SPLIT ? all_kb * (part + 1) / splits : all_kb;   // all_kb <= 1024
 
     if (warp == 0) {
         if (lane == 0) {
@@ -256,14 +258,39 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     } else {
         const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * COLS;
+        // the scales of a tile, asked for one tile ahead
+        constexpr int XS = (COLS + 31) / 32;
+        float xs[XS], ws = 0.f, b = 0.f;
+        auto ask_scales = [&](int t) {
+            const int n0 = (t % ntiles_n) * 128 * CTAS + rank * 128 + quarter * 32 + lane, m0 = (t / ntiles_n) * BN + half * COLS;
+            ws = t < ntiles && n0 < pr.n ? __ldg(pr.w_scale + n0) : 0.f;
+            b = t < ntiles && pr.bias && n0 < pr.n ? __ldg(pr.bias + n0) : 0.f;
+#pragma unroll
+            for (int i = 0; i < XS; i++) xs[i] = t < ntiles && i * 32 + lane < COLS && m0 + i * 32 + lane < pr.m ? __ldg(pr.x_scale + m0 + i * 32 + lane) : 0.f;
+        };
+        ask_scales(worker);
+        if (SPLIT) {   // for the whole CTA, which shares out the columns
+            if (half == 0) {
+                split_w[quarter * 32 + lane] = ws;
+                split_b[quarter * 32 + lane] = b;
+            }
+            if (quarter == 0)
+#pragma unroll
+                for (int i = 0; i < XS; i++)
+                    if (i * 32 + lane < COLS) split_x[half * COLS + i * 32 + lane] = xs[i];
+        }
         int n = 0;
         for (int t = worker; t < ntiles; t += workers, n++) {
             const int a = n & 1;
             const int ch = (t % ntiles_n) * 128 * CTAS + rank * 128 + quarter * 32 + lane, m0 = (t / ntiles_n) * BN + half * COLS;
-            const float ws = ch < pr.n ? pr.w_scale[ch] : 0.f, b = pr.bias && ch < pr.n ? pr.bias[ch] : 0.f;
-            if (!SPLIT) {   // the tile's token scales, while it is being summed
-                for (int c = lane; c < COLS; c += 32) scales[ew][c] = m0 + c < pr.m ? pr.x_scale[m0 + c] : 0.f;
+            const float w_now = ws, b_now = b;
+            if (!SPLIT) {
                 __syncwarp();
+#pragma unroll
+                for (int i = 0; i < XS; i++)
+                    if (i * 32 + lane < COLS) scales[ew][i * 32 + lane] = xs[i];
+                __syncwarp();
+                ask_scales(t + workers);
             }
             if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -283,7 +310,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     // two tokens at a time: the even lane of a pair of channels stores both of one token, the odd lane of the other
 #pragma unroll
                     for (int j = 0; j < CH; j += 2, out += 2 * pr.out_stride) {
-                        float y0 = (float)v[j] * scales[ew][c + j] * ws + b, y1 = (float)v[j + 1] * scales[ew][c + j + 1] * ws + b;
+                        float y0 = (float)v[j] * scales[ew][c + j] * w_now + b_now, y1 = (float)v[j + 1] * scales[ew][c + j + 1] * w_now + b_now;
                         const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? y0 : y1, 1);
                         Pack<T, 2> o;
                         const float f[2] = {lane & 1 ? other : y0, lane & 1 ? y1 : other};
@@ -292,11 +319,11 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     }
                 } else if (whole) {
 #pragma unroll
-                    for (int j = 0; j < CH; j++, out += pr.out_stride) *out = from_float<T>((float)v[j] * scales[ew][c + j] * ws + b);
+                    for (int j = 0; j < CH; j++, out += pr.out_stride) *out = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
                 } else {
 #pragma unroll
                     for (int j = 0; j < CH; j++, out += pr.out_stride) {
-                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>((float)v[j] * scales[ew][c + j] * ws + b);
+                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
                     }
                 }
             }
@@ -309,30 +336,34 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __syncthreads();
     tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all sums are there
     if (SPLIT) {
-        // this CTA's share of the columns: from every CTA of the cluster, 32 neighbouring channels of one token per warp
-        const int share = BN / splits, units = share * 4, t = worker;
-        constexpr int AT_ONCE = 4;   // units of a warp whose loads are in flight together
-        for (int u = warp; u < units; u += AT_ONCE * (LT_THREADS / 32)) {
-            int v[AT_ONCE][8];
-            float xs[AT_ONCE], ws[AT_ONCE], b[AT_ONCE];
+        // this CTA's share of the columns: a warp adds up the 128 channels of a token, four per lane
+        const int share = BN / splits, n0 = (worker % ntiles_n) * 128 + lane * 4, m0 = (worker / ntiles_n) * BN;
+        for (int i = warp; i < share; i += LT_THREADS / 32) {
+            const int col = part * share + i;
+            int4 v[8];
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; i++) {
-                const int unit = u + i * (LT_THREADS / 32), col = part * share + (unit >> 2), l = (unit & 3) * 32 + lane;
-                const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
-                const bool in = unit < units && ch < pr.n && m < pr.m;
+            for (int r = 0; r < 8; r++) v[r] = r < splits ? load_remote(tiles + (uint32_t)(col * 128 + lane * 4) * 4u, r) : make_int4(0, 0, 0, 0);
+            if (m0 + col >= pr.m) continue;
+            int sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int r = 0; r < 8; r++) v[i][r] = unit < units && r < splits ? load_remote(tiles + (uint32_t)(col * 128 + l) * 4u, r) : 0;
-                xs[i] = in ? pr.x_scale[m] : 0.f;
-                ws[i] = in ? pr.w_scale[ch] : 0.f;
-                b[i] = in && pr.bias ? pr.bias[ch] : 0.f;
+            for (int r = 0; r < 8; r++) {
+                sum[0] += v[r].x;
+                sum[1] += v[r].y;
+                sum[2] += v[r].z;
+                sum[3] += v[r].w;
             }
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; i++) {
-                const int unit = u + i * (LT_THREADS / 32), col = part * share + (unit >> 2), l = (unit & 3) * 32 + lane;
-                const int ch = (t % ntiles_n) * 128 + l, m = (t / ntiles_n) * BN + col;
-                const int sum = ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
-                if (unit < units && ch < pr.n && m < pr.m)
-                    ((T *)pr.out)[(long long)m * pr.out_stride + ch] = from_float<T>((float)sum * xs[i] * ws[i] + b[i]);
+            for (int j = 0; j < 4; j++) y[j] = (float)sum[j] * split_x[col] * split_w[lane * 4 + j] + split_b[lane * 4 + j];
+            T *out = (T *)pr.out + (long long)(m0 + col) * pr.out_stride + n0;
+            if (n0 + 4 <= pr.n && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
+                Pack<T, 4> o;
+                pack<4>(o, y);
+                store_pack<T, 4>(out, o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (n0 + j < pr.n) out[j] = from_float<T>(y[j]);
             }
         }
         tile_sync<true>();   // nobody leaves while its sums are read
@@ -400,8 +431,8 @@ template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const Linear
 }
 
 // The tile and the split of k with the least estimated time.  A CTA's stage (128 bytes of k) takes the clocks of its bytes
-// at 64 a clock or of its matrix instructions, whichever is more: 2 (128 + rows of x).  A turn over a tile costs about
-// 1000 clocks more, joining a split one about 3000.
+// at about 52 a clock (measured with 256 rows: 650 clocks) and not less than two copies' own, 470.  A turn over a tile
+// costs about 1000 clocks more, joining a split one about 3000.
 struct TileChoice { int pair, bn, splits; };
 TileChoice choose_tile(const LinearParams &p) {
     const long long sms = sm_count(), kb = (p.k + LT_KB - 1) / LT_KB;
@@ -411,7 +442,7 @@ TileChoice choose_tile(const LinearParams &p) {
         const long long ctas = pair ? 2 : 1, tiles = ((p.n + 128 * ctas - 1) / (128 * ctas)) * ((p.m + bn - 1) / bn);
         if (splits > 1 && (tiles * splits > sms || kb < 2 * splits)) return;
         const long long turns = (tiles * ctas * splits + sms - 1) / sms;
-        const long long cost = turns * ((kb + splits - 1) / splits * 2 * (128 + bn / ctas) + 1000) + (splits > 1 ? 3000 : 0);
+        const long long cost = turns * ((kb + splits - 1) / splits * std::max(470LL, (128 + bn / ctas) * 128 / 50) + 1000) + (splits > 1 ? 3000 : 0);
         if (least < 0 || cost < least) {
             least = cost;
             best = TileChoice{pair, bn, splits};
