@@ -231,16 +231,18 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         auto fill = [&](int g) {
             const T *src = zv + (long long)(v_first + g * (GROUP * TEAM)) * VEC;
             const uint32_t dst = held + (g & 3) * (GROUP * HOP);
+            if (g < groups) {
 #pragma unroll
-            for (int i = 0; i < GROUP; i++) {
-                const int h = g * GROUP + i;
-                if (v_first + h * TEAM < sl.v1) {
-                    copy_async(dst + i * HOP, src + i * (TEAM * VEC), 16);
-                } else if (h < count) {
-                    Pack<T, VEC> none;
+                for (int i = 0; i < GROUP; i++) {
+                    const int h = g * GROUP + i;
+                    if (v_first + h * TEAM < sl.v1) {
+                        copy_async(dst + i * HOP, src + i * (TEAM * VEC), 16);
+                    } else if (h < count) {
+                        Pack<T, VEC> none;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) none.v[e] = from_float<T>(NEG_INF);
-                    store_staged<T, VEC>(dst + i * HOP, none);
+                        for (int e = 0; e < VEC; e++) none.v[e] = from_float<T>(NEG_INF);
+                        store_staged<T, VEC>(dst + i * HOP, none);
+                    }
                 }
             }
             copy_commit();
@@ -413,12 +415,12 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                 }
             }
             if (STATS && scribe && rank == 0) {
-                const double log_s = log((double)sum), log_p = log((double)psum);
+                const double log_s = logf(sum), log_p = logf(psum);   // half a step of about 10 at most: what is added to them is exact
                 double loss = 0;
                 for (int k = lane; k < pr.top; k += 32)
                     if (en.idx[k] >= 0 && en.prob[k] > 0.f)
-                        loss += (double)en.prob[k] * (((double)en.diff[k] - log_p) - (((double)seen(en.own[k]) * (double)c - (double)ref) * 0.6931471805599453 - log_s));
-                loss = warp_sum(loss) / (double)psum;
+                        loss += (double)(en.prob[k] / psum) * (((double)en.diff[k] - log_p) - (((double)seen(en.own[k]) * (double)c - (double)ref) * 0.6931471805599453 - log_s));
+                loss = warp_sum(loss);
                 if (lane == 0) {
                     const double t = pr.temperature;
                     pr.row_loss[row] = (float)(loss * t * t * (double)w * (double)pr.loss_factor);

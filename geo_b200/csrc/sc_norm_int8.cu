@@ -286,16 +286,17 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormPar
     copy_wait<0>();
 }
 
-// One row per CTA at a time, any alignment.  stages: 3, or 1 where three rows do not fit, or 0 (read from memory).
-template <typename T, typename W, bool NORM>
+// One row per CTA at a time, any alignment.  STAGED: rows come through shared memory, `stages` (3, or 1 where three rows do
+// not fit) of them; else from memory, twice.
+template <typename T, typename W, bool NORM, bool STAGED>
 __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, int stages, int buf_bytes) {
+    constexpr int KEEP = 8;   // products of a row that a thread keeps
     extern __shared__ __align__(16) unsigned char norm_smem[];
     __shared__ float part_ss[2][32], part_top[2][32];
     __shared__ double part64[32];
     const int tid = threadIdx.x, threads = blockDim.x, cols = pr.cols;
     const bool has_res = pr.residual != nullptr;
     const T *const x = (const T *)pr.x, *const res = (const T *)pr.residual;
-    T *const sum_out = (T *)pr.sum_out;
     const int stage_bytes = buf_bytes * (has_res ? 2 : 1);
 
     // The 16-byte granules of a row, each at its own distance from the one with the row's first byte.  A granule is read
@@ -320,42 +321,48 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
         }
         copy_commit();
     };
-    if (stages == 3) {
+    if (STAGED && stages == 3) {
         ask(blockIdx.x, 0);
         ask((long long)blockIdx.x + gridDim.x, 1);
     }
     int turn = 0, stage = 0;
     for (long long row = blockIdx.x; row < pr.rows; row += gridDim.x, turn ^= 1) {
-        const T *px = x + row * pr.x_stride, *pq = has_res ? res + row * pr.res_stride : nullptr;
-        if (stages == 3) {
-            ask(row + 2LL * gridDim.x, stage == 0 ? 2 : stage - 1);
-            copy_wait<2>();
-        } else if (stages == 1) {
-            ask(row, 0);
-            copy_wait<0>();
-        }
-        if (stages) {
+        const T *const gx = x + row * pr.x_stride, *const gr = has_res ? res + row * pr.res_stride : nullptr;
+        T *const sum_out = (T *)pr.sum_out + row * cols;
+        const T *sx = nullptr, *sr = nullptr;
+        if (STAGED) {
+            if (stages == 3) {
+                ask(row + 2LL * gridDim.x, stage == 0 ? 2 : stage - 1);
+                copy_wait<2>();
+            } else {
+                ask(row, 0);
+                copy_wait<0>();
+            }
             __syncthreads();
-            px = (const T *)(norm_smem + stage * stage_bytes + ((uintptr_t)px & 15));
-            if (has_res) pq = (const T *)(norm_smem + stage * stage_bytes + buf_bytes + ((uintptr_t)pq & 15));
+            sx = (const T *)(norm_smem + stage * stage_bytes + ((uintptr_t)gx & 15));
+            if (has_res) sr = (const T *)(norm_smem + stage * stage_bytes + buf_bytes + ((uintptr_t)gr & 15));
         }
         auto value = [&](int c) {
-            float r = to_float(px[c]);
-            if (has_res) r = to_float(from_float<T>(r + to_float(pq[c])));
+            float r = to_float(STAGED ? sx[c] : gx[c]);
+            if (has_res) r = to_float(from_float<T>(r + to_float(STAGED ? sr[c] : gr[c])));
             return r;
         };
         auto product = [&](float r, int c) {
             if constexpr (NORM) return r * to_float(((const W *)pr.weight)[c]);
             else return r;
         };
-        float ss = 0.f, top = 0.f;
-#pragma unroll 4
-        for (int c = tid; c < cols; c += threads) {
+        float ss = 0.f, top = 0.f, keep[KEEP];
+        auto take = [&](int c) {
             const float r = value(c);
-            if (has_res) sum_out[row * cols + c] = from_float<T>(r);
+            if (has_res) sum_out[c] = from_float<T>(r);
             if (NORM) ss = fmaf(r, r, ss);
-            top = max_nan(top, fabsf(product(r, c)));
-        }
+            const float p = product(r, c);
+            top = max_nan(top, fabsf(p));
+            return p;
+        };
+#pragma unroll
+        for (int j = 0; j < KEEP; j++) keep[j] = tid + j * threads < cols ? take(tid + j * threads) : 0.f;
+        for (int c = tid + KEEP * threads; c < cols; c += threads) take(c);
         const RowStats st = join_stats<NORM>(ss, top, threads, 0, part_ss, part_top, turn);
         double total = 0;
         if (NORM && st.again) {
@@ -363,16 +370,21 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
             total = join_sum64(total, threads, 0, part64);
         }
         if (tid == 0) pr.scale[row] = row_scale<NORM>(st, total, cols, pr.eps);
-        const bool zero = !(st.top <= 3.402823466e38f) || st.top == 0.f;
-        const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = 127.f / lifted;
-        int8_t *q = pr.q + row * pr.q_stride;
-#pragma unroll 4
-        for (int c = tid; c < cols; c += threads) {
-            const float p[1] = {product(value(c), c) * lift};
-            q[c] = zero ? 0 : round_pack<1>(p, lifted, inv).v[0];
+        const bool fine = st.top <= 3.402823466e38f;
+        const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = fine && st.top > 0.f ? 127.f / lifted : 0.f;
+        int8_t *const q = pr.q + row * pr.q_stride;
+        auto give = [&](float p, int c) {
+            const float v[1] = {fine ? p * lift : 0.f};
+            q[c] = round_pack<1>(v, lifted, inv).v[0];
+        };
+#pragma unroll
+        for (int j = 0; j < KEEP; j++)
+            if (tid + j * threads < cols) give(keep[j], tid + j * threads);
+        for (int c = tid + KEEP * threads; c < cols; c += threads) give(product(value(c), c), c);
+        if (STAGED) {
+            __syncthreads();   // the stage may be overwritten
+            if (stages == 3) stage = stage == 2 ? 0 : stage + 1;
         }
-        if (stages) __syncthreads();   // the stage may be overwritten
-        if (stages == 3) stage = stage == 2 ? 0 : stage + 1;
     }
     copy_wait<0>();
 }
@@ -418,12 +430,14 @@ template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p
     const int stages = stage * 3 <= NORM_SMEM / 2 ? 3 : stage <= NORM_SMEM ? 1 : 0, smem = (int)(stages * stage);
     static PerDeviceOnce once;
     int rc = per_device_once(once, []() -> int {
-        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_ragged_kernel<T, W, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_ragged_kernel<T, W, NORM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
         return GEO_SC_OK;
     });
     if (rc) return rc;
     const long long most = (long long)sm_count() * max(1, min(1024 / threads, smem ? NORM_SMEM / smem : 16));
-    norm_int8_ragged_kernel<T, W, NORM><<<(unsigned)(p.rows < most ? p.rows : most), threads, smem, s>>>(p, stages, (int)buf);
+    const unsigned grid = (unsigned)(p.rows < most ? p.rows : most);
+    if (stages) norm_int8_ragged_kernel<T, W, NORM, true><<<grid, threads, smem, s>>>(p, stages, (int)buf);
+    else norm_int8_ragged_kernel<T, W, NORM, false><<<grid, threads, 0, s>>>(p, 0, 0);
     GEO_CUDA_CHECK(cudaGetLastError());
     return GEO_SC_OK;
 }
