@@ -47,22 +47,21 @@ __device__ __forceinline__ float warp_max_nan(float v) {
     return r;
 }
 
-// VEC products as integers: 127 p / top, half to even; |p| <= top, 1e-30 <= top, finite; inv = 127 / top in fp32.
+// N products as integers: 127 p / top, half to even; |p| <= top, 1e-30 <= top, finite; inv = 127 / top in fp32.
 // p * inv + 1.5 * 2^23 rounds to an integer whose two's complement is the sum's low byte.  Next to a border h between
 // two integers the sign of 127 p - h top decides, whose products are exact in 64 bits.
-template <int VEC> __device__ __forceinline__ Pack<int8_t, VEC> round_pack(const float (&p)[VEC], float top, float inv) {
+template <int N> __device__ __forceinline__ void round_to_top(const float (&p)[N], float top, float inv, uint32_t (&m)[N]) {
     constexpr float MAGIC = 12582912.f, NEAR = 0.5f - 6.2e-5f;
     float off = 0.f;
-    uint32_t m[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
+    for (int e = 0; e < N; e++) {
         const float t = fmaf(p[e], inv, MAGIC);
         off = fmaxf(off, fabsf(fmaf(p[e], inv, MAGIC - t)));
         m[e] = __float_as_uint(t);
     }
     if (off > NEAR) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
+        for (int e = 0; e < N; e++) {
             const float r = __uint_as_float(m[e]) - MAGIC, f = fmaf(p[e], inv, -r);
             if (fabsf(f) > NEAR) {
                 const float h = r + copysignf(0.5f, f);
@@ -71,15 +70,15 @@ template <int VEC> __device__ __forceinline__ Pack<int8_t, VEC> round_pack(const
             }
         }
     }
+}
+template <int VEC> __device__ __forceinline__ Pack<int8_t, VEC> round_pack(const float (&p)[VEC], float top, float inv) {
+    uint32_t m[VEC];
+    round_to_top<VEC>(p, top, inv, m);
     Pack<int8_t, VEC> o;
-    if constexpr (VEC == 1) {
-        o.v[0] = (int8_t)m[0];
-    } else {
-        uint32_t *word = reinterpret_cast<uint32_t *>(&o);
+    uint32_t *word = reinterpret_cast<uint32_t *>(&o);
 #pragma unroll
-        for (int i = 0; i < VEC / 4; i++)
-            word[i] = __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
-    }
+    for (int i = 0; i < VEC / 4; i++)
+        word[i] = __byte_perm(__byte_perm(m[4 * i], m[4 * i + 1], 0x0040), __byte_perm(m[4 * i + 2], m[4 * i + 3], 0x0040), 0x5410);
     return o;
 }
 
@@ -286,18 +285,25 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormPar
     copy_wait<0>();
 }
 
-// One row per CTA at a time, any alignment.  STAGED: rows come through shared memory, `stages` (3, or 1 where three rows do
+// One row per team at a time, a team being a warp (four of them a CTA) or a CTA; any alignment.  STAGED: rows come through shared memory, `stages` (3, or 1 where three rows do
 // not fit) of them; else from memory, twice.
-template <typename T, typename W, bool NORM, bool STAGED>
-__global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, int stages, int buf_bytes) {
+template <typename T, typename W, int THREADS, bool NORM, bool STAGED>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) norm_int8_ragged_kernel(NormParams pr, int stages, int buf_bytes) {
     constexpr int KEEP = 8;   // products of a row that a thread keeps
     extern __shared__ __align__(16) unsigned char norm_smem[];
     __shared__ float part_ss[2][32], part_top[2][32];
     __shared__ double part64[32];
-    const int tid = threadIdx.x, threads = blockDim.x, cols = pr.cols;
+    constexpr int threads = THREADS, TEAMS = THREADS == 32 ? 4 : 1;
+    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, slot = THREADS == 32 ? threadIdx.x >> 5 : 0, cols = pr.cols;
+    auto team_sync = [&]() {
+        if (THREADS == 32) __syncwarp();
+        else __syncthreads();
+    };
     const bool has_res = pr.residual != nullptr;
     const T *const x = (const T *)pr.x, *const res = (const T *)pr.residual;
     const int stage_bytes = buf_bytes * (has_res ? 2 : 1);
+    unsigned char *const bufs = norm_smem + slot * stages * stage_bytes;
+    const long long step = (long long)gridDim.x * TEAMS, start = (long long)blockIdx.x * TEAMS + slot;
 
     // The 16-byte granules of a row, each at its own distance from the one with the row's first byte.  A granule is read
     // from the row's first byte on (value by value) where it begins before it, and up to the row's last byte.
@@ -316,31 +322,31 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
     };
     auto ask = [&](long long row, int stage) {
         if (row < pr.rows) {
-            copy_row(x + row * pr.x_stride, norm_smem + stage * stage_bytes);
-            if (has_res) copy_row(res + row * pr.res_stride, norm_smem + stage * stage_bytes + buf_bytes);
+            copy_row(x + row * pr.x_stride, bufs + stage * stage_bytes);
+            if (has_res) copy_row(res + row * pr.res_stride, bufs + stage * stage_bytes + buf_bytes);
         }
         copy_commit();
     };
     if (STAGED && stages == 3) {
-        ask(blockIdx.x, 0);
-        ask((long long)blockIdx.x + gridDim.x, 1);
+        ask(start, 0);
+        ask(start + step, 1);
     }
     int turn = 0, stage = 0;
-    for (long long row = blockIdx.x; row < pr.rows; row += gridDim.x, turn ^= 1) {
+    for (long long row = start; row < pr.rows; row += step, turn ^= 1) {
         const T *const gx = x + row * pr.x_stride, *const gr = has_res ? res + row * pr.res_stride : nullptr;
         T *const sum_out = (T *)pr.sum_out + row * cols;
         const T *sx = nullptr, *sr = nullptr;
         if (STAGED) {
             if (stages == 3) {
-                ask(row + 2LL * gridDim.x, stage == 0 ? 2 : stage - 1);
+                ask(row + 2 * step, stage == 0 ? 2 : stage - 1);
                 copy_wait<2>();
             } else {
                 ask(row, 0);
                 copy_wait<0>();
             }
-            __syncthreads();
-            sx = (const T *)(norm_smem + stage * stage_bytes + ((uintptr_t)gx & 15));
-            if (has_res) sr = (const T *)(norm_smem + stage * stage_bytes + buf_bytes + ((uintptr_t)gr & 15));
+            team_sync();
+            sx = (const T *)(bufs + stage * stage_bytes + ((uintptr_t)gx & 15));
+            if (has_res) sr = (const T *)(bufs + stage * stage_bytes + buf_bytes + ((uintptr_t)gr & 15));
         }
         auto value = [&](int c) {
             float r = to_float(STAGED ? sx[c] : gx[c]);
@@ -361,7 +367,11 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
             return p;
         };
 #pragma unroll
-        for (int j = 0; j < KEEP; j++) keep[j] = tid + j * threads < cols ? take(tid + j * threads) : 0.f;
+        for (int j = 0; j < KEEP; j++) {
+            keep[j] = 0.f;
+            if ((j + 1) * threads <= cols) keep[j] = take(tid + j * threads);   // the same for every thread
+            else if (tid + j * threads < cols) keep[j] = take(tid + j * threads);
+        }
         for (int c = tid + KEEP * threads; c < cols; c += threads) take(c);
         const RowStats st = join_stats<NORM>(ss, top, threads, 0, part_ss, part_top, turn);
         double total = 0;
@@ -373,16 +383,22 @@ __global__ void __launch_bounds__(1024) norm_int8_ragged_kernel(NormParams pr, i
         const bool fine = st.top <= 3.402823466e38f;
         const float lift = st.top < 1e-30f ? 18446744073709551616.f : 1.f, lifted = st.top * lift, inv = fine && st.top > 0.f ? 127.f / lifted : 0.f;
         int8_t *const q = pr.q + row * pr.q_stride;
-        auto give = [&](float p, int c) {
-            const float v[1] = {fine ? p * lift : 0.f};
-            q[c] = round_pack<1>(v, lifted, inv).v[0];
-        };
+        uint32_t m[KEEP];
+        if (!fine || lift != 1.f)
+#pragma unroll
+            for (int j = 0; j < KEEP; j++) keep[j] = fine ? keep[j] * lift : 0.f;
+        round_to_top<KEEP>(keep, lifted, inv, m);
 #pragma unroll
         for (int j = 0; j < KEEP; j++)
-            if (tid + j * threads < cols) give(keep[j], tid + j * threads);
-        for (int c = tid + KEEP * threads; c < cols; c += threads) give(product(value(c), c), c);
+            if (tid + j * threads < cols) q[tid + j * threads] = (int8_t)m[j];
+        for (int c = tid + KEEP * threads; c < cols; c += threads) {
+            const float p[1] = {fine ? product(value(c), c) * lift : 0.f};
+            uint32_t o[1];
+            round_to_top<1>(p, lifted, inv, o);
+            q[c] = (int8_t)o[0];
+        }
         if (STAGED) {
-            __syncthreads();   // the stage may be overwritten
+            team_sync();   // the stage may be overwritten
             if (stages == 3) stage = stage == 2 ? 0 : stage + 1;
         }
     }
@@ -408,6 +424,24 @@ template <typename T, typename W, int NV, bool NORM> int launch_norm_nv(const No
     return GEO_SC_OK;
 }
 
+template <typename T, typename W, int THREADS, bool NORM> int launch_ragged(const NormParams &p, cudaStream_t s) {
+    constexpr int TEAMS = THREADS == 32 ? 4 : 1, CTA = THREADS * TEAMS;
+    const long long buf = ((long long)p.cols * sizeof(T) + 47) / 16 * 16, stage = buf * (p.residual ? 2 : 1) * TEAMS;
+    const int stages = stage * 3 <= NORM_SMEM / 2 ? 3 : stage <= NORM_SMEM ? 1 : 0, smem = (int)(stages * stage);
+    static PerDeviceOnce once;
+    int rc = per_device_once(once, []() -> int {
+        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_ragged_kernel<T, W, THREADS, NORM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
+        return GEO_SC_OK;
+    });
+    if (rc) return rc;
+    const long long need = (p.rows + TEAMS - 1) / TEAMS, most = (long long)sm_count() * max(1, min(1536 / CTA, smem ? NORM_SMEM / smem : 16));
+    const unsigned grid = (unsigned)(need < most ? need : most);
+    if (stages) norm_int8_ragged_kernel<T, W, THREADS, NORM, true><<<grid, CTA, smem, s>>>(p, stages, (int)buf);
+    else norm_int8_ragged_kernel<T, W, THREADS, NORM, false><<<grid, CTA, 0, s>>>(p, 0, 0);
+    GEO_CUDA_CHECK(cudaGetLastError());
+    return GEO_SC_OK;
+}
+
 template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p, cudaStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
     // whole 16-byte vectors where every row starts on a 16-byte boundary and ends on one
@@ -424,22 +458,10 @@ template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p
         if (nvec <= 2 * tpr) return launch_norm_nv<T, W, 2, NORM>(p, tpr, s);
         return launch_norm_nv<T, W, 4, NORM>(p, tpr, s);
     }
-    int threads = 64;
-    while (threads < 1024 && threads * 8 < p.cols) threads *= 2;
-    const long long buf = ((long long)p.cols * sizeof(T) + 47) / 16 * 16, stage = buf * (p.residual ? 2 : 1);
-    const int stages = stage * 3 <= NORM_SMEM / 2 ? 3 : stage <= NORM_SMEM ? 1 : 0, smem = (int)(stages * stage);
-    static PerDeviceOnce once;
-    int rc = per_device_once(once, []() -> int {
-        GEO_CUDA_CHECK(cudaFuncSetAttribute(norm_int8_ragged_kernel<T, W, NORM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
-        return GEO_SC_OK;
-    });
-    if (rc) return rc;
-    const long long most = (long long)sm_count() * max(1, min(1024 / threads, smem ? NORM_SMEM / smem : 16));
-    const unsigned grid = (unsigned)(p.rows < most ? p.rows : most);
-    if (stages) norm_int8_ragged_kernel<T, W, NORM, true><<<grid, threads, smem, s>>>(p, stages, (int)buf);
-    else norm_int8_ragged_kernel<T, W, NORM, false><<<grid, threads, 0, s>>>(p, 0, 0);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    // eight values per thread, which it keeps in registers, as long as a CTA of 512 goes round
+    if (p.cols <= 256 && p.rows > 1) return launch_ragged<T, W, 32, NORM>(p, s);
+    if (p.cols <= 1024) return launch_ragged<T, W, 128, NORM>(p, s);
+    return p.cols <= 2048 ? launch_ragged<T, W, 256, NORM>(p, s) : launch_ragged<T, W, 512, NORM>(p, s);
 }
 
 // A warp takes STEPS x 32 vectors of a row (read VEC integers, write VEC values), all steps in flight at once.

@@ -13,8 +13,17 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+// through the packed conversions, which are not on the slow conversion pipe
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(0.f), "f"(v));
+    return __ushort_as_bfloat16((unsigned short)r);
+}
+template <> __device__ __forceinline__ __half from_float<__half>(float v) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(0.f), "f"(v));
+    return __ushort_as_half((unsigned short)r);
+}
 
 // N values of T as one load or store (N * sizeof(T) is 16, 8 or 4 bytes, or N = 1).
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };
@@ -69,7 +78,7 @@ template <int N> __device__ __forceinline__ void pack(Pack<float, N> &v, const f
 }
 template <int N> __device__ __forceinline__ void pack(Pack<__nv_bfloat16, N> &v, const float (&f)[N]) {
     if constexpr (N == 1) {
-        v.v[0] = __float2bfloat16_rn(f[0]);
+        v.v[0] = from_float<__nv_bfloat16>(f[0]);
     } else {
         uint32_t *w = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
@@ -78,7 +87,7 @@ template <int N> __device__ __forceinline__ void pack(Pack<__nv_bfloat16, N> &v,
 }
 template <int N> __device__ __forceinline__ void pack(Pack<__half, N> &v, const float (&f)[N]) {
     if constexpr (N == 1) {
-        v.v[0] = __float2half_rn(f[0]);
+        v.v[0] = from_float<__half>(f[0]);
     } else {
         uint32_t *w = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll

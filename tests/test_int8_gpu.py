@@ -40,7 +40,7 @@ def check_norm(x, res, weight, eps, out):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (1, 4096), (5, 512), (300, 64), (700, 257), (33, 2048), (2, 33000), (4, 40000), (400, 1000)])
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 7), (1, 4096), (5, 512), (300, 64), (700, 257), (33, 2048), (2, 33000), (4, 40000), (400, 1000), (500, 255), (50, 2047), (9, 4095), (3, 60001)])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_norm_matches_the_formula(cuda_device, dtype, rows, cols, with_residual):
     from geo_b200 import functional as F
