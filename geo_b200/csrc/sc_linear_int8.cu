@@ -19,8 +19,19 @@ namespace {
 // 16 bytes of a row from byte `at` on, zeros from byte k on.
 __device__ __forceinline__ uint4 load16(const int8_t *row, int at, int k) {
     if (at + 16 <= k) return __ldg((const uint4 *)(row + at));
-    uint32_t v[4] = {0, 0, 0, 0};
-    for (int b = 0; b < 16 && at + b < k; b++) v[b >> 2] |= (uint32_t)(uint8_t)row[at + b] << (8 * (b & 3));
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int b = at + 4 * i;
+        v[i] = 0;
+        if (b + 4 <= k) {
+            v[i] = __ldg((const uint32_t *)(row + b));
+        } else if (b < k) {
+            v[i] = (uint8_t)row[b];
+            if (b + 1 < k) v[i] |= (uint32_t)(uint8_t)row[b + 1] << 8;
+            if (b + 2 < k) v[i] |= (uint32_t)(uint8_t)row[b + 2] << 16;
+        }
+    }
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 

@@ -8,9 +8,10 @@
 // (cta_group::2): each of the pair loads its 128 channels and half of the tokens, the even CTA issues the
 // instructions for both, and each keeps the accumulators of its own channels.
 //
-// Where there are fewer tiles than SMs a cluster of 2, 4 or 8 CTAs shares a tile: each sums a part of k, leaves its
-// integers in its shared memory, and takes a part of the columns over the cluster's shared memory (integers: the order
-// of the additions does not matter).
+// Where there are fewer tiles than SMs a cluster of 2, 4 or 8 CTAs shares a tile: each sums a part of k and sends every
+// column to the shared memory of the CTA that takes it, which adds the parts up behind one barrier of the cluster
+// (integers: the order of the additions does not matter).  Sending costs the sender no waiting; fetching the parts behind
+// the barrier took 3500 clocks more and a second barrier (256 x 4096 x 4096: 18 us).
 //
 // What bounds it: large products the matrix instructions; products of few tokens the bytes that an SM can pull in, about
 // 64 a clock, which is why small tiles on many SMs win over large tiles on few (choose_tile).
@@ -36,11 +37,13 @@ constexpr int LT_EPI_WARPS = 8;
 constexpr int LT_KB = 128;                // bytes of k per stage: one 128-byte swizzled row
 constexpr int LT_SPIN_LIMIT = 1 << 22;
 
-template <int CTAS, int BN> struct LinearTile {
+template <int CTAS, int BN, bool SPLIT> struct LinearTile {
     static constexpr int X_ROWS = BN / CTAS;                                  // token rows that a CTA loads
     static constexpr int STAGE = (128 + X_ROWS) * LT_KB;
-    static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;    // at most 192 KB of tiles
-    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int JOIN = SPLIT ? BN * 128 * 4 : 0;                     // parts of the columns that a CTA takes
+    static constexpr int ROOM = 212 * 1024 - JOIN;
+    static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
+    static constexpr int SMEM = STAGES * STAGE + JOIN + 1024;
     static constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;          // two accumulators
     // kind::i8: 32-bit integers out (2), signed 8-bit A and B (1), both K-major
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CTAS * 128 >> 4) << 24);
@@ -153,12 +156,10 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_ld_wait(int (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS32(LT_INOUT) : : "memory"); }
 __device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_OUT16(LT_INOUT) : : "memory"); }
-__device__ __forceinline__ int4 load_remote(uint32_t addr, int cta) {   // 16 bytes at the same place in another CTA of the cluster
+__device__ __forceinline__ void store_remote(uint32_t addr, int cta, int v) {   // at the same place in another CTA of the cluster
     uint32_t r;
-    int4 v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(cta));
-    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(r) : "memory");
-    return v;
+    asm volatile("st.shared::cluster.b32 [%0], %1;\n" ::"r"(r), "r"(v) : "memory");
 }
 template <bool CLUSTER> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the cluster
     if (!CLUSTER) __syncthreads();
@@ -169,7 +170,7 @@ template <bool CLUSTER> __device__ __forceinline__ void tile_sync() {   // all t
 template <typename T, int CTAS, int BN, bool SPLIT>
 __global__ void __launch_bounds__(LT_THREADS, 1)
 linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearParams pr, int ntiles_n, int ntiles, int splits) {
-    using Tile = LinearTile<CTAS, BN>;
+    using Tile = LinearTile<CTAS, BN, SPLIT>;
     constexpr int ST = Tile::STAGES, COLS = BN / 2;   // columns of an epilogue warp: two warps share a lane quarter
     constexpr int CH = COLS < 32 ? COLS : 32;         // columns read out at a time
     extern __shared__ unsigned char lt_smem_raw[];
@@ -189,6 +190,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     auto accf_bar = [&](int a) { return bar0 + 8u * (2 * ST + a); };
     auto acce_bar = [&](int a) { return bar0 + 8u * (2 * ST + 2 + a); };
     const uint32_t drain_bar = bar0 + 8u * (2 * ST + 4);
+    const uint32_t join = tiles + ST * Tile::STAGE;
+    const int share = SPLIT ? BN / splits : BN;   // columns that a CTA takes: a power of two
     volatile int *abort = &abort_flag;
 
     if (threadIdx.x == 32 * 2) {   // the first copies would wait for these
@@ -206,6 +209,11 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
     tile_sync<CTAS == 2>();
+    // SPLIT: the other CTAs have to have begun before anything is sent to them; every thread waits for that when it can
+    if (SPLIT) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
+    auto cluster_begun = [&]() {
+        if (SPLIT) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    };
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
     const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
@@ -230,6 +238,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             if (!ok && rank == 0)   // the stages that were asked for last
                 for (int i = it < ST ? 0 : it - ST; i < it; i++) mbar_drain(full_bar(i % ST), (i / ST) & 1);
         }
+        __syncwarp();
+        cluster_begun();
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             int it = 0, n = 0;
@@ -255,6 +265,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 mbar_drain(drain_bar, 0);
             }
         }
+        __syncwarp();
+        cluster_begun();
     } else {
         const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * COLS;
@@ -279,6 +291,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 for (int i = 0; i < XS; i++)
                     if (i * 32 + lane < COLS) split_x[half * COLS + i * 32 + lane] = xs[i];
         }
+        cluster_begun();
         int n = 0;
         for (int t = worker; t < ntiles; t += workers, n++) {
             const int a = n & 1;
@@ -302,10 +315,12 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 int v[CH];
                 tmem_ld(lane_addr + a * BN + c, v);
                 tmem_ld_wait(v);
-                if constexpr (SPLIT) {   // columns of 128 lanes; the tiles' shared memory is free (every instruction has read it)
+                if constexpr (SPLIT) {   // [part][column of its taker][128 channels]
 #pragma unroll
-                    for (int j = 0; j < CH; j++)
-                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(tiles + (uint32_t)((half * COLS + c + j) * 128 + quarter * 32 + lane) * 4u), "r"(v[j]) : "memory");
+                    for (int j = 0; j < CH; j++) {
+                        const int col = half * COLS + c + j;
+                        store_remote(join + (uint32_t)((part * share + (col & (share - 1))) * 128 + quarter * 32 + lane) * 4u, col / share, v[j]);
+                    }
                 } else if (whole && sizeof(T) == 2 && paired) {
                     // two tokens at a time: the even lane of a pair of channels stores both of one token, the odd lane of the other
 #pragma unroll
@@ -334,23 +349,21 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all sums are there
+    tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all parts are there
     if (SPLIT) {
-        // this CTA's share of the columns: a warp adds up the 128 channels of a token, four per lane
-        const int share = BN / splits, n0 = (worker % ntiles_n) * 128 + lane * 4, m0 = (worker / ntiles_n) * BN;
+        // a warp adds up the 128 channels of a token, four per lane
+        const int n0 = (worker % ntiles_n) * 128 + lane * 4, m0 = (worker / ntiles_n) * BN;
         for (int i = warp; i < share; i += LT_THREADS / 32) {
             const int col = part * share + i;
-            int4 v[8];
-#pragma unroll
-            for (int r = 0; r < 8; r++) v[r] = r < splits ? load_remote(tiles + (uint32_t)(col * 128 + lane * 4) * 4u, r) : make_int4(0, 0, 0, 0);
             if (m0 + col >= pr.m) continue;
             int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                sum[0] += v[r].x;
-                sum[1] += v[r].y;
-                sum[2] += v[r].z;
-                sum[3] += v[r].w;
+            for (int r = 0; r < splits; r++) {
+                int4 v;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(join + (uint32_t)((r * share + i) * 128 + lane * 4) * 4u));
+                sum[0] += v.x;
+                sum[1] += v.y;
+                sum[2] += v.z;
+                sum[3] += v.w;
             }
             float y[4];
 #pragma unroll
@@ -366,7 +379,6 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     if (n0 + j < pr.n) out[j] = from_float<T>(y[j]);
             }
         }
-        tile_sync<true>();   // nobody leaves while its sums are read
     }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -400,7 +412,7 @@ int encode_rows(CUtensorMap *map, const int8_t *base, int k, int rows, long long
 }
 
 template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const LinearParams &p, int splits, cudaStream_t s) {
-    using Tile = LinearTile<CTAS, BN>;
+    using Tile = LinearTile<CTAS, BN, SPLIT>;
     CUtensorMap map_w, map_x;
     int rc = encode_rows(&map_w, p.w, p.k, p.n, p.w_stride, 128);
     if (!rc) rc = encode_rows(&map_x, p.x, p.k, p.m, p.x_stride, Tile::X_ROWS);
@@ -432,7 +444,7 @@ template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const Linear
 
 // The tile and the split of k with the least estimated time.  A CTA's stage (128 bytes of k) takes the clocks of its bytes
 // at about 52 a clock (measured with 256 rows: 650 clocks) and not less than two copies' own, 470.  A turn over a tile
-// costs about 1000 clocks more, joining a split one about 3000.
+// costs about 1000 clocks more, joining a split one about 2000.
 struct TileChoice { int pair, bn, splits; };
 TileChoice choose_tile(const LinearParams &p) {
     const long long sms = sm_count(), kb = (p.k + LT_KB - 1) / LT_KB;
@@ -442,7 +454,7 @@ TileChoice choose_tile(const LinearParams &p) {
         const long long ctas = pair ? 2 : 1, tiles = ((p.n + 128 * ctas - 1) / (128 * ctas)) * ((p.m + bn - 1) / bn);
         if (splits > 1 && (tiles * splits > sms || kb < 2 * splits)) return;
         const long long turns = (tiles * ctas * splits + sms - 1) / sms;
-        const long long cost = turns * ((kb + splits - 1) / splits * std::max(470LL, (128 + bn / ctas) * 128 / 50) + 1000) + (splits > 1 ? 3000 : 0);
+        const long long cost = turns * ((kb + splits - 1) / splits * std::max(470LL, (128 + bn / ctas) * 128 / 50) + 1000) + (splits > 1 ? 2000 : 0);
         if (least < 0 || cost < least) {
             least = cost;
             best = TileChoice{pair, bn, splits};
