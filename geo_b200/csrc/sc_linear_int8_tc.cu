@@ -135,27 +135,18 @@ template <int CTAS> __device__ __forceinline__ void tmem_free(uint32_t base, uin
     if (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
 }
-#define LT_REGS32(x) x(0), x(1), x(2), x(3), x(4), x(5), x(6), x(7), x(8), x(9), x(10), x(11), x(12), x(13), x(14), x(15), x(16), x(17), x(18), x(19), x(20), x(21), x(22), x(23), x(24), x(25), x(26), x(27), x(28), x(29), x(30), x(31)
 #define LT_OUT(i) "=r"(r[i])
 #define LT_INOUT(i) "+r"(r[i])
-#define LT_OUT16(x) x(0), x(1), x(2), x(3), x(4), x(5), x(6), x(7), x(8), x(9), x(10), x(11), x(12), x(13), x(14), x(15)
-// N columns of the warp's 32 lanes; the registers may be read after tmem_ld_wait (they pass through it, so that nothing
+#define LT_REGS16(x) x(0), x(1), x(2), x(3), x(4), x(5), x(6), x(7), x(8), x(9), x(10), x(11), x(12), x(13), x(14), x(15)
+// 16 columns of the warp's 32 lanes; the registers may be read after tmem_ld_wait (they pass through it, so that nothing
 // that reads them moves up).
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-                 : LT_REGS32(LT_OUT)
-                 : "r"(taddr)
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-                 : LT_OUT16(LT_OUT)
+                 : LT_REGS16(LT_OUT)
                  : "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait(int (&r)[32]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS32(LT_INOUT) : : "memory"); }
-__device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_OUT16(LT_INOUT) : : "memory"); }
+__device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS16(LT_INOUT) : : "memory"); }
 __device__ __forceinline__ void store_remote(uint32_t addr, int cta, int v) {   // at the same place in another CTA of the cluster
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(cta));
@@ -172,7 +163,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1)
 linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearParams pr, int ntiles_n, int ntiles, int splits) {
     using Tile = LinearTile<CTAS, BN, SPLIT>;
     constexpr int ST = Tile::STAGES, COLS = BN / 2;   // columns of an epilogue warp: two warps share a lane quarter
-    constexpr int CH = COLS < 32 ? COLS : 32;         // columns read out at a time
+    constexpr int CH = 16;                            // columns read out at a time
     extern __shared__ unsigned char lt_smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * ST + 5];   // full, empty, acc_full[2], acc_empty[2], drain
     __shared__ __align__(16) float scales[LT_EPI_WARPS][COLS];
@@ -310,11 +301,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             T *out = (T *)pr.out + (long long)m0 * pr.out_stride + ch;
             const bool paired = pr.out_stride % 2 == 0 && ((uintptr_t)pr.out & 3) == 0;
             const bool whole = !SPLIT && ch - lane + 32 <= pr.n && m0 + COLS <= pr.m;
-#pragma unroll 1
-            for (int c = 0; c < COLS; c += CH) {
-                int v[CH];
-                tmem_ld(lane_addr + a * BN + c, v);
-                tmem_ld_wait(v);
+            auto process = [&](const int (&v)[CH], int c) {
                 if constexpr (SPLIT) {   // [part][column of its taker][128 channels]
 #pragma unroll
                     for (int j = 0; j < CH; j++) {
@@ -323,23 +310,43 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     }
                 } else if (whole && sizeof(T) == 2 && paired) {
                     // two tokens at a time: the even lane of a pair of channels stores both of one token, the odd lane of the other
+                    T *at = lane & 1 ? out + pr.out_stride - 1 : out;
 #pragma unroll
-                    for (int j = 0; j < CH; j += 2, out += 2 * pr.out_stride) {
-                        float y0 = (float)v[j] * scales[ew][c + j] * w_now + b_now, y1 = (float)v[j + 1] * scales[ew][c + j + 1] * w_now + b_now;
+                    for (int j = 0; j < CH; j += 2, at += 2 * pr.out_stride) {
+                        const float y0 = (float)v[j] * scales[ew][c + j] * w_now + b_now, y1 = (float)v[j + 1] * scales[ew][c + j + 1] * w_now + b_now;
                         const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? y0 : y1, 1);
                         Pack<T, 2> o;
                         const float f[2] = {lane & 1 ? other : y0, lane & 1 ? y1 : other};
                         pack<2>(o, f);
-                        store_pack<T, 2>(lane & 1 ? out + pr.out_stride - 1 : out, o);
+                        store_pack<T, 2>(at, o);
                     }
                 } else if (whole) {
+                    T *at = out;
 #pragma unroll
-                    for (int j = 0; j < CH; j++, out += pr.out_stride) *out = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
+                    for (int j = 0; j < CH; j++, at += pr.out_stride) *at = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
                 } else {
+                    T *at = out;
 #pragma unroll
-                    for (int j = 0; j < CH; j++, out += pr.out_stride) {
-                        if (ch < pr.n && m0 + c + j < pr.m) *out = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
-                    }
+                    for (int j = 0; j < CH; j++, at += pr.out_stride)
+                        if (ch < pr.n && m0 + c + j < pr.m) *at = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
+                }
+                out += CH * pr.out_stride;
+            };
+            // the next columns are read out of tensor memory while these are stored
+            int va[CH], vb[CH];
+            tmem_ld(lane_addr + a * BN, va);
+            if constexpr (COLS == CH) {
+                tmem_ld_wait(va);
+                process(va, 0);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < COLS; c += 2 * CH) {
+                    tmem_ld_wait(va);
+                    tmem_ld(lane_addr + a * BN + c + CH, vb);
+                    process(va, c);
+                    tmem_ld_wait(vb);
+                    if (c + 2 * CH < COLS) tmem_ld(lane_addr + a * BN + c + 2 * CH, va);
+                    process(vb, c + CH);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
