@@ -147,10 +147,10 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&r)[16]) {
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait(int (&r)[16]) { asm volatile("tcgen05.wait::ld.sync.aligned;\n" : LT_REGS16(LT_INOUT) : : "memory"); }
-__device__ __forceinline__ void store_remote(uint32_t addr, int cta, int v) {   // at the same place in another CTA of the cluster
+__device__ __forceinline__ void store_remote(uint32_t addr, int cta, int a, int b, int c, int d) {   // at the same place in another CTA of the cluster
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(cta));
-    asm volatile("st.shared::cluster.b32 [%0], %1;\n" ::"r"(r), "r"(v) : "memory");
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(r), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 template <bool CLUSTER> __device__ __forceinline__ void tile_sync() {   // all threads of the CTA, or of the cluster
     if (!CLUSTER) __syncthreads();
@@ -299,16 +299,16 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             T *out = (T *)pr.out + (long long)m0 * pr.out_stride + ch;
-            const bool paired = pr.out_stride % 2 == 0 && ((uintptr_t)pr.out & 3) == 0;
-            const bool whole = !SPLIT && ch - lane + 32 <= pr.n && m0 + COLS <= pr.m;
+            const bool paired = sizeof(T) == 2 && pr.out_stride % 2 == 0 && pr.n % 2 == 0 && ((uintptr_t)pr.out & 3) == 0;
+            const int tokens = min(COLS, pr.m - m0);   // of this warp's columns
             auto process = [&](const int (&v)[CH], int c) {
-                if constexpr (SPLIT) {   // [part][column of its taker][128 channels]
+                if constexpr (SPLIT) {   // [part][four columns of their taker][128 channels][column]
 #pragma unroll
-                    for (int j = 0; j < CH; j++) {
+                    for (int j = 0; j < CH; j += 4) {
                         const int col = half * COLS + c + j;
-                        store_remote(join + (uint32_t)((part * share + (col & (share - 1))) * 128 + quarter * 32 + lane) * 4u, col / share, v[j]);
+                        store_remote(join + (uint32_t)(((part * share + (col & (share - 1))) >> 2) * 128 + quarter * 32 + lane) * 16u, col / share, v[j], v[j + 1], v[j + 2], v[j + 3]);
                     }
-                } else if (whole && sizeof(T) == 2 && paired) {
+                } else if (c + CH <= tokens && paired) {
                     // two tokens at a time: the even lane of a pair of channels stores both of one token, the odd lane of the other
                     T *at = lane & 1 ? out + pr.out_stride - 1 : out;
 #pragma unroll
@@ -318,17 +318,20 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                         Pack<T, 2> o;
                         const float f[2] = {lane & 1 ? other : y0, lane & 1 ? y1 : other};
                         pack<2>(o, f);
-                        store_pack<T, 2>(at, o);
+                        if (ch < pr.n) store_pack<T, 2>(at, o);
                     }
-                } else if (whole) {
+                } else if (c + CH <= tokens) {
                     T *at = out;
 #pragma unroll
-                    for (int j = 0; j < CH; j++, at += pr.out_stride) *at = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
-                } else {
+                    for (int j = 0; j < CH; j++, at += pr.out_stride) {
+                        const T y = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
+                        if (ch < pr.n) *at = y;
+                    }
+                } else if (c < tokens) {
                     T *at = out;
 #pragma unroll
                     for (int j = 0; j < CH; j++, at += pr.out_stride)
-                        if (ch < pr.n && m0 + c + j < pr.m) *at = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
+                        if (ch < pr.n && c + j < tokens) *at = from_float<T>((float)v[j] * scales[ew][c + j] * w_now + b_now);
                 }
                 out += CH * pr.out_stride;
             };
@@ -358,33 +361,24 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __syncthreads();
     tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all parts are there
     if (SPLIT) {
-        // a warp adds up the 128 channels of a token, four per lane
-        const int n0 = (worker % ntiles_n) * 128 + lane * 4, m0 = (worker / ntiles_n) * BN;
-        for (int i = warp; i < share; i += LT_THREADS / 32) {
-            const int col = part * share + i;
-            if (m0 + col >= pr.m) continue;
+        // a warp adds up 32 channels of four tokens
+        const int n0 = (worker % ntiles_n) * 128, m0 = (worker / ntiles_n) * BN + part * share;
+        for (int i = warp; i < share; i += LT_THREADS / 32) {   // share / 4 groups of tokens x 4 of channels
+            const int group = i >> 2, l = (i & 3) * 32 + lane, ch = n0 + l, m = m0 + group * 4;
+            if (m >= pr.m || ch >= pr.n) continue;
             int sum[4] = {0, 0, 0, 0};
             for (int r = 0; r < splits; r++) {
                 int4 v;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(join + (uint32_t)((r * share + i) * 128 + lane * 4) * 4u));
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(join + (uint32_t)((((r * share) >> 2) + group) * 128 + l) * 16u));
                 sum[0] += v.x;
                 sum[1] += v.y;
                 sum[2] += v.z;
                 sum[3] += v.w;
             }
-            float y[4];
+            T *out = (T *)pr.out + (long long)m * pr.out_stride + ch;
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = (float)sum[j] * split_x[col] * split_w[lane * 4 + j] + split_b[lane * 4 + j];
-            T *out = (T *)pr.out + (long long)(m0 + col) * pr.out_stride + n0;
-            if (n0 + 4 <= pr.n && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
-                Pack<T, 4> o;
-                pack<4>(o, y);
-                store_pack<T, 4>(out, o);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (n0 + j < pr.n) out[j] = from_float<T>(y[j]);
-            }
+            for (int j = 0; j < 4; j++, out += pr.out_stride)
+                if (m + j < pr.m) *out = from_float<T>((float)sum[j] * split_x[part * share + group * 4 + j] * split_w[l] + split_b[l]);
         }
     }
     if (warp == 1) {
