@@ -250,17 +250,17 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         auto fill_all = [&]() {
             for (int g = 0; g < 4; g++) fill(g);
         };
-        // f(vector, its place in shared memory) for every vector, when it has arrived; `resident`: all of them have, and stay
-        auto each = [&](bool resident, auto f) {
+        // all_of(first vector, its place) for groups that every lane has all of, one(vector, its place) for the other vectors,
+        // when they have arrived; `resident`: all of them have, and stay
+        auto each = [&](bool resident, auto all_of, auto one) {
             for (int g = 0; g < groups; g++) {
                 if (!resident) copy_wait<3>();
                 const uint32_t at = held + (g & 3) * (GROUP * HOP);
                 if (g < whole) {
-#pragma unroll
-                    for (int i = 0; i < GROUP; i++) f(g * GROUP + i, at + i * HOP, std::true_type());
+                    all_of(g * GROUP, at);
                 } else {
 #pragma unroll 1
-                    for (int i = 0; i < GROUP && g * GROUP + i < count; i++) f(g * GROUP + i, at + i * HOP, std::false_type());
+                    for (int i = 0; i < GROUP && g * GROUP + i < count; i++) one(g * GROUP + i, at + i * HOP);
                 }
                 if (!resident) fill(g + 4);
             }
@@ -296,20 +296,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             constexpr bool FLAT = decltype(is_flat)::value;
             float top = r_at >= 0 ? seen(r_value) : NEG_INF, ref = scaled(top), base = base_of(ref), s1 = 0.f;
             float s0 = r_at >= 0 ? ex2(fmaf(top, c, -base)) : 0.f;
-            each(FLAT && groups <= 4, [&](int, uint32_t at, auto) {
-                const Pack<T, VEC> v = load_staged<T, VEC>(at);
-                float f[VEC], large;
-                unpack<VEC>(v, f);
-                if (FLAT) {
-                    large = NEG_INF;
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        f[e] = seen(f[e]);
-                        large = fmaxf(large, f[e]);
-                    }
-                } else {
-                    large = pack_max<VEC>(v);
-                }
+            auto look = [&](float large) {
                 top = fmaxf(top, large);
                 if (scaled(large) > ref + 32.f) {
                     const float to_ref = scaled(large);
@@ -318,12 +305,46 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                     ref = to_ref;
                     base = base_of(ref);
                 }
+            };
+            auto add = [&](const float (&f)[VEC]) {
 #pragma unroll
                 for (int e = 0; e < VEC; e += 2) {
                     s0 += ex2(fmaf(f[e], c, -base));
                     s1 += ex2(fmaf(f[e + 1], c, -base));
                 }
-            });
+            };
+            auto one = [&](int, uint32_t at) {
+                float f[VEC], large = NEG_INF;
+                unpack<VEC>(load_staged<T, VEC>(at), f);
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    if (FLAT) f[e] = seen(f[e]);
+                    large = fmaxf(large, f[e]);
+                }
+                look(large);
+                add(f);
+            };
+            each(FLAT && groups <= 4, [&](int h, uint32_t at) {
+                if (FLAT) {
+#pragma unroll 1
+                    for (int i = 0; i < GROUP; i++) one(h + i, at + i * HOP);
+                } else {
+                    Pack<T, VEC> v[GROUP];
+                    float large = NEG_INF;
+#pragma unroll
+                    for (int i = 0; i < GROUP; i++) {
+                        v[i] = load_staged<T, VEC>(at + i * HOP);
+                        large = fmaxf(large, pack_max<VEC>(v[i]));
+                    }
+                    look(large);
+#pragma unroll
+                    for (int i = 0; i < GROUP; i++) {
+                        float f[VEC];
+                        unpack<VEC>(v[i], f);
+                        add(f);
+                    }
+                }
+            }, one);
             most = warp_max(top);
             total = warp_sum(moved(s0 + s1, ref, scaled(most)));
         };
@@ -360,17 +381,50 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             }
             if (m == NEG_INF) sum = __int_as_float(0x7fc00000);   // no logit above -inf: no distribution
         } else {
-            team_sync();
             m = pr.stats[row].x;
             sum = pr.stats[row].y;
             flat = out_of_range();
+        }
+        const float ref = flat ? 0.f : scaled(m), inv_s = 1.f / sum, a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, a_s = a * inv_s;
+        const bool wide = GRAD && ((uintptr_t)(grad + sl.head) & 15) == 0;
+        auto give_all = [&]() {   // the gradient apart from the teacher's share
+            if (!wide) {   // the rows of the gradient lie otherwise in memory than those of the logits
+                for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
+                return;
+            }
+            const bool resident = STATS && groups <= 4;
+            if (STATS && !resident) fill_all();
+            T *out = grad + sl.head + (long long)v_first * VEC;
+            auto give = [&](auto is_flat) {
+                auto share = [&](uint32_t at) {
+                    float f[VEC];
+                    unpack<VEC>(load_staged<T, VEC>(at), f);
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) f[e] = ex2(fmaf(decltype(is_flat)::value ? seen(f[e]) : f[e], c, -ref)) * a_s;
+                    Pack<T, VEC> o;
+                    pack<VEC>(o, f);
+                    return o;
+                };
+                each(resident, [&](int h, uint32_t at) {
+#pragma unroll
+                    for (int i = 0; i < GROUP; i++) store_pack<T, VEC>(out + (long long)(h + i) * (TEAM * VEC), share(at + i * HOP));
+                }, [&](int h, uint32_t at) {
+                    const Pack<T, VEC> o = share(at);
+                    if (v_first + h * TEAM < sl.v1) store_pack<T, VEC>(out + (long long)h * (TEAM * VEC), o);
+                });
+            };
+            if (flat) give(std::true_type());
+            else give(std::false_type());
+            if (r_at >= 0) grad[r_at] = from_float<T>(ex2(fmaf(seen(r_value), c, -ref)) * a_s);
+        };
+        if (!STATS) {   // before the entries are known: a thread writes the same places again where the row turns out to have none
+            if (GRAD && streams) give_all();
+            team_sync();
         }
         if (TEAM > 32) {
             state = row_state;
             psum = row_psum;
         }
-        const float ref = flat ? 0.f : scaled(m);
-        const bool wide = GRAD && ((uintptr_t)(grad + sl.head) & 15) == 0;
 
         if (state) {   // the same for every CTA of a cluster
             const float v = state == 1 ? 0.f : __int_as_float(0x7fc00000);
@@ -390,30 +444,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                 }
             }
         } else {
-            const float a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, inv_s = 1.f / sum, a_s = a * inv_s;
-            if (GRAD && streams) {
-                if (wide) {
-                    const bool resident = STATS && groups <= 4;
-                    if (STATS && !resident) fill_all();
-                    T *out = grad + sl.head + (long long)v_first * VEC;
-                    auto give = [&](auto is_flat) {
-                        each(resident, [&](int h, uint32_t at, auto all_lanes) {
-                            float f[VEC];
-                            unpack<VEC>(load_staged<T, VEC>(at), f);
-#pragma unroll
-                            for (int e = 0; e < VEC; e++) f[e] = ex2(fmaf(decltype(is_flat)::value ? seen(f[e]) : f[e], c, -ref)) * a_s;
-                            Pack<T, VEC> o;
-                            pack<VEC>(o, f);
-                            if (decltype(all_lanes)::value || v_first + h * TEAM < sl.v1) store_pack<T, VEC>(out + (long long)h * (TEAM * VEC), o);
-                        });
-                    };
-                    if (flat) give(std::true_type());
-                    else give(std::false_type());
-                    if (r_at >= 0) grad[r_at] = from_float<T>(ex2(fmaf(seen(r_value), c, -ref)) * a_s);
-                } else {   // the rows of the gradient lie otherwise in memory than those of the logits
-                    for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
-                }
-            }
+            if (STATS && GRAD && streams) give_all();
             if (STATS && scribe && rank == 0) {
                 const double log_s = logf(sum), log_p = logf(psum);   // half a step of about 10 at most: what is added to them is exact
                 double loss = 0;
@@ -428,7 +459,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                 }
             }
             if (GRAD) {
-                team_sync();   // the entries' places are written a second time, after the pass above
+                if (STATS) team_sync();   // the entries' places are written a second time, after the pass above
                 for (int k = tid; k < pr.top; k += TEAM == 32 ? 32 : TEAM + 32)
                     if (en.merged[k] >= 0.f) grad[en.idx[k]] = from_float<T>((ex2(fmaf(seen(en.own[k]), c, -ref)) * inv_s - en.merged[k]) * a);
             }
