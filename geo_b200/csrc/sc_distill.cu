@@ -95,9 +95,9 @@ __host__ __device__ constexpr int held_vectors(bool grad) { return grad ? 16 : 8
 constexpr int DISTILL_SMEM = 200 * 1024;   // of an SM's 227 KB
 // a team's shared memory: 20 bytes per entry, the table that finds entries of the same index, then the team's vectors
 __host__ __device__ inline int table_slots(int top) {
-    int n = 32;
+    int n = 64;
     while (n < 2 * top) n *= 2;
-    return n;
+    return top <= 32 ? 0 : n;
 }
 __host__ __device__ inline int entry_room(int top) { return (top * 20 + table_slots(top) * 4 + 15) / 16 * 16; }
 
@@ -112,65 +112,88 @@ struct Entries {
     int slots;
 };
 // 0: a row with entries, 1: without (or of weight 0), 2: with a bad entry.
-template <typename T, bool GRAD>
-__device__ __forceinline__ int take_entries(const DistillParams &pr, const Entries &en, long long row, const T *z, float w, float inv_t, int from, int to, float &psum) {
+template <typename T, int AT_ONCE>   // AT_ONCE: entries of a lane whose loads are in flight together, the index, then the logit that it names
+__device__ __forceinline__ int take_entries(const DistillParams &pr, const Entries &en, long long row, const T *z, float w, float inv_t, float &psum) {
     const int lane = threadIdx.x & 31;
     float tmax = NEG_INF;
     bool bad = false;
-    if (GRAD)
-        for (int i = lane; i < en.slots; i += 32) en.table[i] = -1;
-    for (int k = lane; k < pr.top; k += 32) {
-        const long long at = row * pr.top + k;
-        const long long j = pr.index64 ? ((const long long *)pr.indices)[at] : ((const int *)pr.indices)[at];
-        const float t = teacher_at(pr, at);
-        const bool use = j >= 0, fits = use && j < pr.vocab;
-        bad |= use && (!fits || !(t < INFINITY));
-        en.idx[k] = fits ? (int)j : -1;
-        en.own[k] = fits ? to_float(z[j]) : 0.f;
-        en.diff[k] = use ? t : NEG_INF;
-        if (use) tmax = fmaxf(tmax, t);
+    for (int first = lane; first < pr.top; first += 32 * AT_ONCE) {
+        long long j[AT_ONCE];
+        float t[AT_ONCE], own[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int k = first + i * 32;
+            const long long at = row * pr.top + k;
+            j[i] = k >= pr.top ? -1 : pr.index64 ? ((const long long *)pr.indices)[at] : ((const int *)pr.indices)[at];
+            t[i] = k >= pr.top ? NEG_INF : teacher_at(pr, at);
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) own[i] = j[i] >= 0 && j[i] < pr.vocab ? to_float(z[j[i]]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int k = first + i * 32;
+            const bool use = j[i] >= 0, fits = use && j[i] < pr.vocab;
+            bad |= use && (!fits || !(t[i] < INFINITY));
+            if (use) tmax = fmaxf(tmax, t[i]);
+            if (k < pr.top) {
+                en.idx[k] = fits ? (int)j[i] : -1;
+                en.own[k] = own[i];
+                en.diff[k] = use ? t[i] : NEG_INF;
+            }
+        }
     }
     bad = __any_sync(0xffffffffu, bad);
     tmax = warp_max(tmax);
     if (w == 0.f || (!bad && tmax == NEG_INF)) return 1;
     if (bad) return 2;
     psum = 0.f;
-    bool twice = false;
-    __syncwarp();   // the table is clear
     for (int k = lane; k < pr.top; k += 32) {
         const float d = (en.diff[k] - tmax) * inv_t, e = expf(d);
         en.diff[k] = d;
         en.prob[k] = e;
         psum += e;
-        const int j = en.idx[k];
-        if (GRAD && j >= 0) {   // open addressing; at most half of the slots are ever taken
-            for (int i = (unsigned)j * 2654435769u >> 16;; i++) {
+    }
+    psum = warp_sum(psum);
+    return 0;
+}
+
+// The probability that an index in [from, to) carries, with its first entry.
+__device__ __forceinline__ void merge_entries(const Entries &en, int top, int from, int to, float psum) {
+    const int lane = threadIdx.x & 31;
+    bool twice = false;
+    if (top <= 32) {
+        const int j = lane < top ? en.idx[lane] : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, j);
+        twice = j >= 0 && (same & (same - 1)) != 0;
+    } else {
+        for (int i = lane; i < en.slots; i += 32) en.table[i] = -1;
+        __syncwarp();
+        for (int k = lane; k < top; k += 32) {
+            const int j = en.idx[k];
+            if (j < 0) continue;
+            for (int i = (unsigned)j * 2654435769u >> 16;; i++) {   // open addressing; at most half of the slots are ever taken
                 const int was = atomicCAS(&en.table[i & (en.slots - 1)], -1, j);
                 twice |= was == j;
                 if (was == -1 || was == j) break;
             }
         }
     }
-    psum = warp_sum(psum);
-    if (GRAD) {
-        twice = __any_sync(0xffffffffu, twice);
-        __syncwarp();
-        for (int k = lane; k < pr.top; k += 32) {
-            const int j = en.idx[k];
-            bool first = j >= from && j < to;
-            float p = en.prob[k];
-            if (twice && first) {
-                p = 0.f;
-                for (int i = 0; i < pr.top; i++)
-                    if (en.idx[i] == j) {
-                        p += en.prob[i];
-                        first &= i >= k;
-                    }
-            }
-            en.merged[k] = first ? p / psum : -1.f;
+    twice = __any_sync(0xffffffffu, twice);
+    __syncwarp();
+    for (int k = lane; k < top; k += 32) {
+        const int j = en.idx[k];
+        bool first = j >= from && j < to;
+        float p = en.prob[k];
+        if (twice && first) {
+            p = 0.f;
+            for (int i = 0; i < top; i++)
+                if (en.idx[i] == j) {
+                    p += en.prob[i];
+                    first &= i >= k;
+                }
         }
+        en.merged[k] = first ? p / psum : -1.f;
     }
-    return 0;
 }
 
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER>
@@ -277,7 +300,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         int state = 0;
         float psum = 1.f;
         if (scribe) {
-            state = take_entries<T, GRAD>(pr, en, row, z, w, inv_t, from, to, psum);
+            state = take_entries<T, TEAM == 32 ? 1 : 4>(pr, en, row, z, w, inv_t, psum);
             if (TEAM > 32 && lane == 0) {
                 row_state = state;
                 row_psum = psum;
@@ -419,6 +442,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         };
         if (!STATS) {   // before the entries are known: a thread writes the same places again where the row turns out to have none
             if (GRAD && streams) give_all();
+            if (GRAD && scribe && state == 0) merge_entries(en, pr.top, from, to, psum);
             team_sync();
         }
         if (TEAM > 32) {
@@ -445,6 +469,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             }
         } else {
             if (STATS && GRAD && streams) give_all();
+            if (STATS && GRAD && scribe) merge_entries(en, pr.top, from, to, psum);
             if (STATS && scribe && rank == 0) {
                 const double log_s = logf(sum), log_p = logf(psum);   // half a step of about 10 at most: what is added to them is exact
                 double loss = 0;

@@ -12,9 +12,9 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 def reference(logits, indices, teacher, T, weight, scale, up):
     """(row losses, gradient, bound of the losses' error, bound of the gradient's) in 64 bits; `up` per row.
 
-    Bounds: an exponential's argument is off by three half steps of itself (difference, product, constant; 2^-22.4 |a|
-    with |a| below 64 / 1.44 in what carries a sum: 2^-17), ex2 by 2^-22, a sum of up to 2^17 terms by 2^-17 (256 terms
-    one after the other in a thread, then joined): 2^-15 covers q, p and their logarithms' absolute error."""
+    Bounds: an exponential's argument is off by some half steps of itself (product, constant; 2^-22 |a| with |a| below 64
+    in what carries a sum: 2^-16), ex2 by 2^-22, a sum of up to 2^17 terms by 2^-17 (at most 512 terms one after the
+    other in a thread, then joined): 2^-15 covers q, p and their logarithms' absolute error."""
     z, w = logits.detach().cpu().double(), (torch.ones(logits.shape[0]) if weight is None else weight.cpu()).double()
     idx, t = indices.cpu().long(), teacher.cpu().double() / T
     t = torch.where(idx >= 0, t, -math.inf)
@@ -163,9 +163,9 @@ def test_bad_entries_poison_their_row_only(cuda_device, vocab):
     assert abs(float(mean) - float(clean[4:].double().mean())) <= 1e-6 * abs(float(mean))
 
 
-@pytest.mark.parametrize("vocab", [20, 1200])
-def test_one_index_several_times(cuda_device, vocab):
-    logits, indices, teacher = make(5, vocab, 12, torch.float32, 9, cuda_device)
+@pytest.mark.parametrize("vocab, top", [(20, 12), (1200, 12), (1200, 33), (1200, 512), (50000, 300)])
+def test_one_index_several_times(cuda_device, vocab, top):
+    logits, indices, teacher = make(5, vocab, top, torch.float32, 9, cuda_device)
     indices[:, 3] = indices[:, 0]
     indices[:, 7] = indices[:, 0]
     indices[:, 11] = indices[:, 5]
@@ -233,6 +233,17 @@ def test_second_backward_and_accumulation(cuda_device):
     assert torch.equal(logits.grad, (kept.float() * 2).bfloat16())
     with torch.no_grad():
         assert not F.distillation_loss(logits, indices, teacher).requires_grad
+
+
+def test_differentiable_once(cuda_device):
+    from geo_b200 import functional as F
+
+    logits, indices, teacher = make(4, 30, 5, torch.float32, 2, cuda_device)
+    (grad,) = torch.autograd.grad(F.distillation_loss(logits, indices, teacher), logits, create_graph=True)
+    (plain,) = torch.autograd.grad(F.distillation_loss(logits, indices, teacher), logits)
+    assert torch.equal(grad, plain)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
 
 
 def test_captured_and_on_another_stream(cuda_device):
