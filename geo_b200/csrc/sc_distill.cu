@@ -198,6 +198,7 @@ __device__ __forceinline__ void merge_entries(const Entries &en, int top, int fr
 
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER>
 __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) distill_kernel(DistillParams pr, int team_bytes) {
+    if (!STATS && pr.skip_one && !pr.upstream_rows && pr.upstream[0] == 1.f) return;   // the whole gradient is there already
     constexpr int VEC = 16 / sizeof(T), WARPS = TEAM / 32, HOP = TEAM * 16;   // bytes between a thread's vectors
     constexpr int GROUP = held_vectors(GRAD) / 4;
     extern __shared__ __align__(16) unsigned char distill_smem[];

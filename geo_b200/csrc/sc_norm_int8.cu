@@ -448,12 +448,14 @@ template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p
     const bool wide = p.cols % VEC == 0 && aligned_to(p.x, 16) && p.x_stride % VEC == 0 && (!p.residual || (aligned_to(p.residual, 16) && p.res_stride % VEC == 0)) &&
                       (!p.sum_out || aligned_to(p.sum_out, 16)) && aligned_to(p.q, VEC) && p.q_stride % VEC == 0 && (!NORM || aligned_to(p.weight, 16));
     if (wide) {
-        // few rows: one vector per thread, the shortest way through a row; many: four, for a quarter of the reductions
-        // (16384 rows of 8192 fp16 values: with two vectors 220 us, of 320 instructions per vector two thirds per row)
+        // Few rows: one vector per thread, the shortest way through a row.  Many: two per thread for rows of up to 256
+        // vectors (8192 x 1024 fp32 with read-back 30.0 us, with four 32.6), four for longer ones, which have fewer
+        // reductions then (16384 x 8192 fp16: 227 us, with two 235).
         const int nvec = p.cols / VEC;
         const bool few = p.rows < 2LL * sm_count() && nvec <= 1024;
+        const int most = few ? 1024 : 512, want = few ? nvec : nvec <= 256 ? (nvec + 1) / 2 : (nvec + 3) / 4;
         int tpr = 32;
-        while (tpr < (few ? 1024 : 512) && tpr < (few ? nvec : (nvec + 3) / 4)) tpr *= 2;
+        while (tpr < most && tpr < want) tpr *= 2;
         if (nvec <= tpr) return launch_norm_nv<T, W, 1, NORM>(p, tpr, s);
         if (nvec <= 2 * tpr) return launch_norm_nv<T, W, 2, NORM>(p, tpr, s);
         return launch_norm_nv<T, W, 4, NORM>(p, tpr, s);
