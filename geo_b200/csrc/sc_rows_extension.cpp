@@ -4,6 +4,7 @@
 // for two microseconds on the device: what a call costs is what the host spends on it.
 //
 // Arguments are checked before the device is looked at, so that a wrong shape is named on a machine without a GPU too.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -78,10 +79,15 @@ Tensor rows_of(const Tensor &t) {
     return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
 
+// Uninitialised output on the device, past the dispatcher (a third of what an allocation costs the host).
+Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, at::Device device) {
+    return at::detail::empty_cuda(sizes, dtype, device, std::nullopt);
+}
+
 // int8 [rows, cols] whose rows start on 16-byte boundaries, as the product reads them.
 Tensor empty_rows(int64_t rows, int64_t cols, at::Device device) {
     const int64_t padded = (cols + 15) / 16 * 16;
-    const Tensor t = at::empty({rows, padded}, at::TensorOptions().dtype(at::kChar).device(device));
+    const Tensor t = new_tensor({rows, padded}, at::kChar, device);
     return padded == cols ? t : t.narrow(1, 0, cols);
 }
 
@@ -93,8 +99,6 @@ Tensor aligned_rows(const Tensor &t) {
 Tensor like_rows(const Tensor &q, const Tensor &x) {   // [rows, cols] back to the leading dimensions of x
     return x.dim() == 2 ? q : x.dim() == 1 ? q.select(0, 0) : q.unflatten(0, x.sizes().slice(0, x.dim() - 1));
 }
-
-at::TensorOptions floats(const Tensor &like) { return like.options().dtype(at::kFloat).requires_grad(false); }
 
 py::tuple rms_norm_int8(const Tensor &x, const Tensor &weight, const OptTensor &residual_, double eps) {
     const Tensor *residual = ptr(residual_);
@@ -114,11 +118,11 @@ py::tuple rms_norm_int8(const Tensor &x, const Tensor &weight, const OptTensor &
     const Tensor xr = rows_of(x), w = (weight.scalar_type() == x.scalar_type() ? weight : weight.to(at::kFloat)).contiguous();
     const int wcode = dtype_code(w.scalar_type(), "weight");
     const int64_t rows = xr.size(0);
-    const Tensor q = empty_rows(rows, cols, x.device()), scale = at::empty(x.sizes().slice(0, x.dim() - 1), floats(x));
+    const Tensor q = empty_rows(rows, cols, x.device()), scale = new_tensor(x.sizes().slice(0, x.dim() - 1), at::kFloat, x.device());
     Tensor rr, total;
     if (residual) {
         rr = rows_of(*residual);
-        total = at::empty(x.sizes(), x.options().requires_grad(false));
+        total = new_tensor(x.sizes(), x.scalar_type(), x.device());
     }
     check(geo_sc_rms_norm_int8(rows, (int)cols, code, xr.data_ptr(), xr.stride(0), residual ? rr.data_ptr() : nullptr,
                                residual ? rr.stride(0) : 0, w.data_ptr(), wcode, (float)eps, residual ? total.data_ptr() : nullptr,
@@ -136,7 +140,7 @@ py::tuple quantize_int8(const Tensor &x) {
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor xr = rows_of(x);
-    const Tensor q = empty_rows(xr.size(0), xr.size(1), x.device()), scale = at::empty(x.sizes().slice(0, x.dim() - 1), floats(x));
+    const Tensor q = empty_rows(xr.size(0), xr.size(1), x.device()), scale = new_tensor(x.sizes().slice(0, x.dim() - 1), at::kFloat, x.device());
     check(geo_sc_quantize_int8(xr.size(0), (int)xr.size(1), code, xr.data_ptr(), xr.stride(0), (int8_t *)q.data_ptr(), q.stride(0),
                                (float *)scale.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
           "geo_sc_quantize_int8");
@@ -154,7 +158,7 @@ Tensor dequantize_int8(const Tensor &q, const Tensor &scale, at::ScalarType dtyp
     one_device({&q, &scale});
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(q.device());
-    const Tensor qr = rows_of(q), s = scale.contiguous(), out = at::empty(q.sizes(), q.options().dtype(dtype));
+    const Tensor qr = rows_of(q), s = scale.contiguous(), out = new_tensor(q.sizes(), dtype, q.device());
     check(geo_sc_dequantize_int8(qr.size(0), (int)qr.size(1), (const int8_t *)qr.data_ptr(), qr.stride(0), (const float *)s.data_ptr(), code,
                                  out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
           "geo_sc_dequantize_int8");
@@ -191,7 +195,7 @@ Tensor linear_int8(const Tensor &q, const Tensor &scale, const Tensor &weight_q,
     const int64_t m = x.size(0);
     at::DimVector shape(q.sizes());
     shape.back() = n;
-    const Tensor out = at::empty(shape, q.options().dtype(dtype));
+    const Tensor out = new_tensor(shape, dtype, q.device());
     check(geo_sc_linear_int8((int)m, (int)n, (int)k, (const int8_t *)x.data_ptr(), x.stride(0), (const float *)s.data_ptr(),
                              (const int8_t *)w.data_ptr(), w.stride(0), (const float *)ws.data_ptr(), bias ? (const float *)b.data_ptr() : nullptr,
                              code, out.data_ptr(), n, c10::cuda::getCurrentCUDAStream().stream()),
@@ -210,11 +214,11 @@ struct Distillation : torch::autograd::Function<Distillation> {
         c10::cuda::CUDAGuard guard(logits.device());
         const Tensor z = rows_of(logits);
         const int64_t rows = z.size(0), vocab = z.size(1);
-        const Tensor row_loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), floats(logits));
-        const Tensor stats = at::empty({rows, 2}, floats(logits));
+        const Tensor row_loss = new_tensor(logits.sizes().slice(0, logits.dim() - 1), at::kFloat, logits.device());
+        const Tensor stats = new_tensor({rows, 2}, at::kFloat, logits.device());
         Tensor loss, grad;
-        if (mean) loss = at::empty({}, floats(logits));
-        if (mean && need) grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
+        if (mean) loss = new_tensor({}, at::kFloat, logits.device());
+        if (mean && need) grad = new_tensor(logits.sizes(), logits.scalar_type(), logits.device());
         check(geo_sc_distill_forward(rows, (int)vocab, (int)indices.size(-1), dtype_code(logits.scalar_type(), "logits"), z.data_ptr(),
                                      z.stride(0), indices.data_ptr(), indices.scalar_type() == at::kLong ? 64 : 32, teacher.data_ptr(),
                                      dtype_code(teacher.scalar_type(), "teacher_logits"),
@@ -249,7 +253,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
                 ctx->saved_data.erase(it);
                 ready = true;
             } else {
-                grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
+                grad = new_tensor(logits.sizes(), logits.scalar_type(), logits.device());
             }
             check(geo_sc_distill_backward(z.size(0), (int)z.size(1), (int)indices.size(-1), dtype_code(logits.scalar_type(), "logits"),
                                           z.data_ptr(), z.stride(0), indices.data_ptr(), indices.scalar_type() == at::kLong ? 64 : 32,
