@@ -3,6 +3,8 @@ hand-written CUDA for NVIDIA B200 (sm_100a), behind the reference's own operator
 
     geo_b200.functional   conv2d_generic / linear_generic / quantize   (utils_functional.py)
     geo_b200.layers       Conv2d_Add_Partial, BatchNorm2d_fixed, ...   (utils_class.py)
+                          and, beside them, 8-bit evaluation (rms_norm_int8, linear_int8, ...: layers.RMSNorm_Int8,
+                          layers.Linear_Int8) and distillation_loss (layers.DistillationLoss)
     geo_b200.network      CONV_tiny_add_partial, VGG11_add_partial     (network.py)
     geo_b200.ops          torch front end of the C ABI (include/geo_sc.h)
     geo_b200.ext          sc_extension_cuda / sc_extension pybind11 modules (reference names)

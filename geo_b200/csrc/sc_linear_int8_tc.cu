@@ -11,10 +11,12 @@
 // Where there are fewer tiles than SMs a cluster of 2, 4 or 8 CTAs shares a tile: each sums a part of k and sends every
 // column to the shared memory of the CTA that takes it, which adds the parts up behind one barrier of the cluster
 // (integers: the order of the additions does not matter).  Sending costs the sender no waiting; fetching the parts behind
-// the barrier took 3500 clocks more and a second barrier (256 x 4096 x 4096: 18 us).
+// the barrier took 3500 clocks more and a second barrier (256 x 4096 x 4096: 18 us against 12).
 //
-// What bounds it: large products the matrix instructions; products of few tokens the bytes that an SM can pull in, about
-// 64 a clock, which is why small tiles on many SMs win over large tiles on few (choose_tile).
+// What bounds it: the bytes that an SM takes in, about 50 a clock (a pair's stage of 32 KB per CTA takes 650 clocks, its
+// matrix instructions 512), which is why a pair shares its tokens and why small tiles on many SMs win over large tiles on
+// few (choose_tile).  Measured: 8192 x 8192 x 8192 358 us = 3070 TOP/s (415 us under the power limit), 1024 x 4096 x 4096
+// 16 us, 256 x 4096 x 4096 12 us, 333 x 1001 x 2047 8.4 us.
 //
 // Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
 // out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the
