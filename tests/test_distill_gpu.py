@@ -65,7 +65,8 @@ def check(logits, indices, teacher, T=1.0, weight=None, scale=1.0, up=None, redu
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows, vocab, top", [(1, 1, 1), (256, 10, 3), (5, 2, 2), (9, 100, 100), (33, 1000, 17), (3, 1024, 512), (3, 1025, 40),
-                                              (400, 1500, 8), (7, 4099, 64), (2, 33333, 100), (1, 131071, 256), (200, 8192, 31)])
+                                              (400, 1500, 8), (7, 4099, 64), (2, 33333, 100), (1, 131071, 256), (200, 8192, 31),
+                                              (600, 33333, 9), (3, 300001, 20)])
 def test_loss_and_gradient_match_the_formula(cuda_device, dtype, rows, vocab, top):
     logits, indices, teacher = make(rows, vocab, top, dtype, rows + vocab, cuda_device)
     g = torch.Generator().manual_seed(1)
@@ -124,7 +125,7 @@ def test_masked_logits(cuda_device, dtype, vocab):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("vocab", [41, 3000, 90001])
+@pytest.mark.parametrize("vocab", [41, 3000, 90001, 300001])
 def test_rows_at_the_ends_of_the_type(cuda_device, dtype, vocab):
     """Rows masked by the type's lowest value throughout, or in part by -inf, and rows around the largest value: whatever
     the temperature, logits that are equal have equal probabilities and the others none."""
@@ -196,6 +197,30 @@ def test_strides_and_shapes(cuda_device, dtype):
     loss.backward()
     assert float(loss) == 0 and empty.grad.shape == (0, 2000)
     assert F.distillation_loss(empty, indices[:0], teacher[:0], reduction="none").shape == (0,)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """66000 rows of 33000 logits are more than 2^31 values: the last rows as a call of their own gives them."""
+    from geo_b200 import functional as F
+
+    rows, vocab, last = 66000, 33000, 5
+    logits = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=cuda_device)
+    g = torch.Generator().manual_seed(6)
+    logits[-last:] = torch.randn(last, vocab, generator=g).bfloat16().to(cuda_device)
+    logits.requires_grad_(True)
+    indices = torch.randint(0, vocab, (rows, 4), generator=g).to(cuda_device)
+    teacher = torch.randn(rows, 4, generator=g).to(cuda_device)
+    small = logits.detach()[-last:].clone().requires_grad_(True)
+    expect = F.distillation_loss(small, indices[-last:], teacher[-last:], 2.0, reduction="none")
+    (expect_grad,) = torch.autograd.grad(expect.sum(), small)
+    loss = F.distillation_loss(logits, indices, teacher, 2.0, reduction="none")
+    (grad,) = torch.autograd.grad(loss.sum(), logits)
+    # another team may hold the rows there: the same values but for the order of a sum
+    assert (loss[-last:] - expect).abs().max() <= 2.0 ** -18 * expect.abs().max()
+    assert (grad[-last:].float() - expect_grad.float()).abs().max() <= 2.0 ** -8 * expect_grad.float().abs().max()
+    scalar = F.distillation_loss(logits, indices, teacher, 2.0, reduction="sum")
+    (grad,) = torch.autograd.grad(scalar, logits)
+    assert (grad[-last:].float() - expect_grad.float()).abs().max() <= 2.0 ** -8 * expect_grad.float().abs().max()
 
 
 def test_gradient_against_differences(cuda_device):

@@ -230,6 +230,29 @@ def test_product_writes_its_rows_only(cuda_device):
         assert (out[m:] == -7).all() and (out[:, n:] == -7).all()
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 values in rows, integers and outputs: the last rows are right."""
+    from geo_b200 import functional as F
+
+    for cols in (16400, 16401):
+        x = torch.zeros(131100, cols, dtype=torch.bfloat16, device=cuda_device)
+        g = torch.Generator().manual_seed(cols)
+        x[-3:] = torch.randn(3, cols, generator=g).bfloat16().to(cuda_device)
+        q, scale = F.quantize_int8(x)
+        expect, _ = reference_rows(x[-3:].cpu(), None)
+        assert torch.equal(q[-3:].cpu(), expect) and (q[:2] == 0).all()
+        y = F.dequantize_int8(q, scale, torch.bfloat16)
+        exact = q[-3:].cpu().double() * scale[-3:].cpu().double()[:, None]
+        assert ((y[-3:].cpu().double() - exact).abs() <= exact.abs() * (2.0 ** -8 + 2.0 ** -20)).all()
+        del x, y
+    m, n = 70000, 33001
+    x, w = int8_rows(g, m, 32, cuda_device), int8_rows(g, n, 32, cuda_device)
+    xs, ws = torch.rand(m, generator=g).to(cuda_device), torch.rand(n, generator=g).to(cuda_device)
+    out = F.linear_int8(x, xs, w, ws, dtype=torch.bfloat16)
+    check_product(x[-300:], xs[-300:], w, ws, None, out[-300:])
+    check_product(x[:7], xs[:7], w, ws, None, out[:7])
+
+
 def test_layers_chain_and_capture(cuda_device):
     """norm -> 8-bit layer -> residual -> norm -> 8-bit layer, eagerly, on another stream and replayed from a graph."""
     from geo_b200 import layers
