@@ -196,19 +196,26 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         for (int s = 0; s < ST; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < 2; a++) { mbar_init(accf_bar(a), 1); mbar_init(acce_bar(a), LT_EPI_WARPS * CTAS); }
         mbar_init(drain_bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;\n" ::: "memory");
     }
     if (warp == 1) tmem_alloc<CTAS>(smem_u32(&tmem_slot), Tile::TMEM_COLS);
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-    __syncthreads();
-    tile_sync<CTAS == 2>();
+    if (CTAS == 2) {
+        __syncthreads();
+        tile_sync<true>();
+    } else if (warp == 0) {   // the first copies need the barriers only, which this warp has made: it does not wait for the others
+        __syncwarp();
+        asm volatile("barrier.cta.arrive.aligned 1, %0;\n" ::"n"(LT_THREADS) : "memory");
+    } else {
+        asm volatile("barrier.cta.sync.aligned 1, %0;\n" ::"n"(LT_THREADS) : "memory");
+    }
     // SPLIT: the other CTAs have to have begun before anything is sent to them; every thread waits for that when it can
-    if (SPLIT) asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
+    if (SPLIT) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
     auto cluster_begun = [&]() {
         if (SPLIT) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
     };
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    const uint32_t tmem_base = tmem_slot;
+    const uint32_t tmem_base = CTAS == 1 && warp == 0 ? 0 : tmem_slot;   // not that warp's to read
     const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
     const int kb0 = SPLIT ? all_kb * part / splits : 0, kb1 = SPLIT ? all_kb * (part + 1) / splits : all_kb;   // all_kb <= 1024
 
