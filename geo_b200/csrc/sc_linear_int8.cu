@@ -12,7 +12,7 @@
 // the same 16 bytes of its token rows for two instructions: whole 16-byte loads, no shared memory, no shuffles.  A CTA
 // of eight warps owns 16 channels x 8 * NT tokens; the warps split k and join their integer sums in shared memory.
 // Bound by the weights' bytes: 1 x 8192 x 8192 15.4 us (4.4 TB/s with the launch), 16 x 4096 x 4096 4.7 us.  Above 32
-// tokens the other kernel takes less (64 x 4096 x 4096: 8.1 us; 32 tokens: 6.7 here, 11.5 there).
+// tokens the other kernel takes less (64 x 4096 x 4096: 7.9 us; 32 tokens: 6.6 here, 6.9 there).
 #include "sc_linear_int8.h"
 
 namespace geo {

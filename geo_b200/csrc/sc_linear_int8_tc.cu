@@ -15,8 +15,8 @@
 //
 // What bounds it: the bytes that an SM takes in, about 50 a clock (a pair's stage of 32 KB per CTA takes 650 clocks, its
 // matrix instructions 512), which is why a pair shares its tokens and why small tiles on many SMs win over large tiles on
-// few (choose_tile).  Measured: 8192 x 8192 x 8192 358 us = 3070 TOP/s (415 us under the power limit), 1024 x 4096 x 4096
-// 16 us, 256 x 4096 x 4096 12 us, 333 x 1001 x 2047 8.4 us.
+// few as long as one turn holds them (choose_tile).  Measured: 8192 x 8192 x 8192 361 us = 3045 TOP/s (415 us under the power limit), 1024 x 4096 x 4096
+// 16 us, 256 x 4096 x 4096 12 us, 333 x 1001 x 2047 7.9 us.
 //
 // Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
 // out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the
@@ -452,27 +452,31 @@ template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const Linear
     return GEO_SC_OK;
 }
 
-// The tile and the split of k with the least estimated time.  A CTA's stage (128 bytes of k) takes the clocks of its bytes
-// at about 52 a clock (measured with 256 rows: 650 clocks) and not less than two copies' own, 470.  A turn over a tile
-// costs about 1000 clocks more, joining a split one about 2000.
+// The tile and the split of k with the least estimated time, in units of 10 ns.  Measured over products of 12 to 2000
+// tokens (CUDA-graph replay): a call with one turn takes `start` and `stage` for each 128 bytes of k, whatever the number
+// of CTAs; every further turn its stages and 0.6 us, or the stores of a tile (`stores`) where they take longer; sending
+// and joining the parts of a split tile takes `join`.  So small tiles win while a turn holds them all (123 x 1920 x 944:
+// 32 tokens 6.0 us, 128 tokens 7.4, a pair 8.6), large ones when there are several (378 x 6812 x 3765: a pair 15.3 us,
+// 64 tokens 30.6), and a split of k pays where few tiles have a long k (50 x 500 x 8000: 6.8 us by 8, 21.0 whole).
 struct TileChoice { int pair, bn, splits; };
+struct TileTimes { int pair, bn, start, stage, stores, join; };
 TileChoice choose_tile(const LinearParams &p) {
+    constexpr TileTimes TIMES[] = {{0, 32, 340, 28, 90, 130}, {0, 64, 350, 29, 130, 200}, {0, 128, 430, 31, 250, 290}, {1, 256, 560, 32, 340, 0}};
     const long long sms = sm_count(), kb = (p.k + LT_KB - 1) / LT_KB;
     TileChoice best{0, 64, 1};
     long long least = -1;
-    auto consider = [&](int pair, int bn, int splits) {
-        const long long ctas = pair ? 2 : 1, tiles = ((p.n + 128 * ctas - 1) / (128 * ctas)) * ((p.m + bn - 1) / bn);
-        if (splits > 1 && (tiles * splits > sms || kb < 2 * splits)) return;
-        const long long turns = (tiles * ctas * splits + sms - 1) / sms;
-        const long long cost = turns * ((kb + splits - 1) / splits * std::max(470LL, (128 + bn / ctas) * 128 / 50) + 1000) + (splits > 1 ? 2000 : 0);
-        if (least < 0 || cost < least) {
-            least = cost;
-            best = TileChoice{pair, bn, splits};
+    for (const TileTimes &t : TIMES) {
+        const long long ctas = t.pair ? 2 : 1, tiles = ((p.n + 128 * ctas - 1) / (128 * ctas)) * ((p.m + t.bn - 1) / t.bn);
+        for (int splits = 1; splits <= (t.pair ? 1 : 8); splits *= 2) {
+            if (splits > 1 && (tiles * splits > sms || kb < 2 * splits)) break;
+            const long long turns = (tiles * ctas * splits + sms - 1) / sms, stages = (kb + splits - 1) / splits * t.stage;
+            const long long cost = t.start + stages + (turns - 1) * std::max(stages + 60, (long long)t.stores) + (splits > 1 ? t.join : 0);
+            if (least < 0 || cost < least) {
+                least = cost;
+                best = TileChoice{t.pair, t.bn, splits};
+            }
         }
-    };
-    consider(1, 256, 1);
-    for (int bn = 128; bn >= 32; bn /= 2)
-        for (int splits = 1; splits <= 8; splits *= 2) consider(0, bn, splits);
+    }
     return best;
 }
 

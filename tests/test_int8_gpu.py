@@ -159,7 +159,8 @@ def check_product(x, xs, w, ws, bias, out):
 PRODUCT_SIZES = [(1, 1, 1), (1, 16, 16), (1, 4096, 1024), (2, 33, 65), (7, 100, 2047), (8, 64, 64), (9, 129, 333), (17, 64, 4097),
                  (32, 48, 128), (33, 257, 100), (65, 130, 1000), (100, 10, 512), (128, 128, 128), (129, 127, 255), (256, 512, 512),
                  (300, 1001, 130), (513, 511, 640), (1000, 64, 33), (64, 2048, 2048), (700, 900, 1),
-                 (100, 19000, 64), (129, 9500, 70), (257, 9600, 130), (1000, 5000, 300), (2000, 2100, 1024), (300, 20000, 16)]
+                 (100, 19000, 64), (129, 9500, 70), (257, 9600, 130), (1000, 5000, 300), (2000, 2100, 1024), (300, 20000, 16),
+                 (200, 300, 4000), (50, 500, 8000), (400, 900, 6000), (450, 401, 9001), (600, 701, 3001), (1100, 1501, 700)]
 
 
 @pytest.mark.parametrize("m, n, k", PRODUCT_SIZES)
