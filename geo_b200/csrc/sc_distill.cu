@@ -199,6 +199,8 @@ __device__ __forceinline__ void merge_entries(const Entries &en, int top, int fr
 
 template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER>
 __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) distill_kernel(DistillParams pr, int team_bytes) {
+    ahead_of_previous();
+    after_previous();
     if (!STATS && pr.skip_one && !pr.upstream_rows && pr.upstream[0] == 1.f) return;   // the whole gradient is there already
     constexpr int VEC = 16 / sizeof(T), WARPS = TEAM / 32, HOP = TEAM * 16;   // bytes between a thread's vectors
     constexpr int GROUP = held_vectors(GRAD) / 4;
@@ -499,6 +501,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
 // The rows' losses as one value, in a fixed order.
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const float *row_loss, long long rows, double factor, float *loss) {
     __shared__ double part[32];
+    ahead_of_previous();
+    after_previous();
     double s = 0;
     for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)row_loss[i];
     s = warp_sum(s);
@@ -516,28 +520,17 @@ template <typename T, int TEAM, bool STATS, bool GRAD, bool CLUSTER> int launch_
     // a pass that may have nothing to do is not worth a CTA for every row: as many as are resident, walking over the rows
     const long long resident = (long long)sm_count() * team_blocks(TEAM, GRAD) / ranks;
     if ((p.skip_one || grid * ranks > 0x7fffffffLL) && grid > resident) grid = resident;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(grid * ranks));
-    cfg.blockDim = dim3(threads);
     const long long per_cta = ((long long)p.vocab * (long long)sizeof(T) / 16 + ranks - 1) / ranks;   // vectors of a CTA's slice at most
     // whole warps of vectors: the lanes past a slice have a place too
     const int team_bytes = entry_room(p.top) + (int)(per_cta < TEAM * held_vectors(GRAD) ? (per_cta + 31) / 32 * 32 : TEAM * held_vectors(GRAD)) * 16;
-    cfg.dynamicSmemBytes = (size_t)(TEAM == 32 ? 4 : 1) * team_bytes;
     static PerDeviceOnce once;
     int rc = per_device_once(once, []() -> int {
         GEO_CUDA_CHECK(cudaFuncSetAttribute(distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, DISTILL_SMEM));
         return GEO_SC_OK;
     });
     if (rc) return rc;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = CLUSTER ? 1 : 0;
-    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, p, team_bytes));
-    return GEO_SC_OK;
+    return launch_behind(distill_kernel<T, TEAM, STATS, GRAD, CLUSTER>, (unsigned)(grid * ranks), threads, (size_t)(TEAM == 32 ? 4 : 1) * team_bytes, s, ranks, p,
+                         team_bytes);
 }
 
 template <typename T, bool STATS, bool GRAD> int launch_distill(const DistillParams &p, cudaStream_t s) {
@@ -596,8 +589,7 @@ int geo_sc_distill_forward(long long rows, int vocab, int top, int dtype, const 
         if (rc) return rc;
     }
     if (mean) {
-        distill_sum_kernel<<<1, 1024, 0, s>>>(row_loss, rows, all, loss);
-        GEO_CUDA_CHECK(cudaGetLastError());
+        return launch_behind(distill_sum_kernel, 1, 1024, 0, s, 1, (const float *)row_loss, rows, all, loss);
     }
     return GEO_SC_OK;
 }

@@ -48,6 +48,8 @@ constexpr int MMA_WARPS = 8;
 template <typename T, int NT>
 __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearParams p) {
     __shared__ int sums[MMA_WARPS][NT * 8][16];
+    ahead_of_previous();
+    after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int mtiles = (p.m + NT * 8 - 1) / (NT * 8);
     const int m0 = (int)(blockIdx.x % mtiles) * NT * 8, n0 = (int)(blockIdx.x / mtiles) * 16;
@@ -123,11 +125,8 @@ template <typename T> int launch_mma(const LinearParams &p, cudaStream_t s) {
     const int nt = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
     const long long grid = (long long)((p.m + nt * 8 - 1) / (nt * 8)) * ((p.n + 15) / 16);
     if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
-    if (nt == 1) linear_int8_mma_kernel<T, 1><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
-    else if (nt == 2) linear_int8_mma_kernel<T, 2><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
-    else linear_int8_mma_kernel<T, 4><<<(unsigned)grid, 32 * MMA_WARPS, 0, s>>>(p);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    const auto kernel = nt == 1 ? linear_int8_mma_kernel<T, 1> : nt == 2 ? linear_int8_mma_kernel<T, 2> : linear_int8_mma_kernel<T, 4>;
+    return launch_behind(kernel, (unsigned)grid, 32 * MMA_WARPS, 0, s, 1, p);
 }
 
 }  // namespace

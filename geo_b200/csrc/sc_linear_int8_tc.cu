@@ -187,6 +187,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const int share = SPLIT ? BN / splits : BN;   // columns that a CTA takes: a power of two
     volatile int *abort = &abort_flag;
 
+    ahead_of_previous();
     if (threadIdx.x == 32 * 2) {   // the first copies would wait for these
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map_x) : "memory");
@@ -217,6 +218,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem_base = CTAS == 1 && warp == 0 ? 0 : tmem_slot;   // not that warp's to read
     const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
+    after_previous();
     const int kb0 = SPLIT ? all_kb * part / splits : 0, kb1 = SPLIT ? all_kb * (part + 1) / splits : all_kb;   // all_kb <= 1024
 
     if (warp == 0) {
@@ -437,19 +439,7 @@ template <typename T, int CTAS, int BN, bool SPLIT> int launch_tile(const Linear
     const long long tiles = (long long)tn * ((p.m + BN - 1) / BN);
     if (tiles > 0x3fffffff) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
     const int workers = SPLIT ? (int)tiles : (int)(tiles < sm_count() / CTAS ? tiles : sm_count() / CTAS), cluster = SPLIT ? splits : CTAS;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(workers * cluster));
-    cfg.blockDim = dim3(LT_THREADS);
-    cfg.dynamicSmemBytes = Tile::SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_int8_tc_kernel<T, CTAS, BN, SPLIT>, map_w, map_x, p, tn, (int)tiles, splits));
-    return GEO_SC_OK;
+    return launch_behind(linear_int8_tc_kernel<T, CTAS, BN, SPLIT>, (unsigned)(workers * cluster), LT_THREADS, Tile::SMEM, s, cluster, map_w, map_x, p, tn, (int)tiles, splits);
 }
 
 // The tile and the split of k with the least estimated time, in units of 10 ns.  Measured over products of 12 to 2000

@@ -148,6 +148,7 @@ __device__ __forceinline__ double join_sum64(double v, int tpr, int first, doubl
 template <typename T, typename W, int NV, bool NORM>
 __global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormParams pr, int tpr) {
     constexpr int VEC = 16 / sizeof(T), STAGES = 3;
+    ahead_of_previous();
     extern __shared__ __align__(16) unsigned char norm_smem[];
     __shared__ float part_ss[2][32], part_top[2][32];
     __shared__ double part64[32];
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormPar
         next_x += step * pr.x_stride;
         next_r += step * pr.res_stride;
     };
+    after_previous();
     ask(start, 0);
     ask(start + step, 1);
     int turn = 0, stage = 0;
@@ -292,6 +294,7 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_int8_kernel(NormPar
 template <typename T, typename W, int THREADS, bool NORM, bool STAGED>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) norm_int8_ragged_kernel(NormParams pr, int stages, int buf_bytes) {
     constexpr int KEEP = 8;   // products of a row that a thread keeps
+    ahead_of_previous();
     extern __shared__ __align__(16) unsigned char norm_smem[];
     __shared__ float part_ss[2][32], part_top[2][32];
     __shared__ double part64[32];
@@ -329,6 +332,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) norm_int8_ragge
         }
         copy_commit();
     };
+    after_previous();
     if (STAGED && stages == 3) {
         ask(start, 0);
         ask(start + step, 1);
@@ -421,9 +425,7 @@ template <typename T, typename W, int NV, bool NORM> int launch_norm_nv(const No
     // as many CTAs as fit every SM's registers and the stages
     const int per_sm = max(1, min((NV == 4 ? 512 : 1024) / threads, NORM_SMEM / smem));
     const long long need = (p.rows + rpc - 1) / rpc, most = (long long)sm_count() * per_sm;
-    norm_int8_kernel<T, W, NV, NORM><<<(unsigned)(need < most ? need : most), threads, smem, s>>>(p, tpr);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    return launch_behind(norm_int8_kernel<T, W, NV, NORM>, (unsigned)(need < most ? need : most), threads, smem, s, 1, p, tpr);
 }
 
 template <typename T, typename W, int THREADS, bool NORM> int launch_ragged(const NormParams &p, cudaStream_t s) {
@@ -438,10 +440,8 @@ template <typename T, typename W, int THREADS, bool NORM> int launch_ragged(cons
     if (rc) return rc;
     const long long need = (p.rows + TEAMS - 1) / TEAMS, most = (long long)sm_count() * max(1, min(1536 / CTA, smem ? NORM_SMEM / smem : 16));
     const unsigned grid = (unsigned)(need < most ? need : most);
-    if (stages) norm_int8_ragged_kernel<T, W, THREADS, NORM, true><<<grid, CTA, smem, s>>>(p, stages, (int)buf);
-    else norm_int8_ragged_kernel<T, W, THREADS, NORM, false><<<grid, CTA, 0, s>>>(p, 0, 0);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    if (stages) return launch_behind(norm_int8_ragged_kernel<T, W, THREADS, NORM, true>, grid, CTA, smem, s, 1, p, stages, (int)buf);
+    return launch_behind(norm_int8_ragged_kernel<T, W, THREADS, NORM, false>, grid, CTA, 0, s, 1, p, 0, 0);
 }
 
 template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p, cudaStream_t s) {
@@ -472,6 +472,8 @@ template <typename T, typename W, bool NORM> int launch_norm(const NormParams &p
 template <typename T, int VEC, int STEPS>
 __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t *q, long long q_stride, const float *scale, T *out, long long units, int upr,
                                                                int nvec, int cols) {
+    ahead_of_previous();
+    after_previous();
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (unit >= units) return;
     const long long row = units <= 0xffffffffLL ? (long long)((unsigned)unit / (unsigned)upr) : unit / upr;
@@ -505,9 +507,7 @@ template <typename T, int VEC, int STEPS> int launch_dequantize_v(long long rows
     const int nvec = cols / VEC, upr = (nvec + 32 * STEPS - 1) / (32 * STEPS);
     const long long units = rows * upr, grid = (units + 7) / 8;
     if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%lld rows of %d values", rows, cols);
-    dequantize_int8_kernel<T, VEC, STEPS><<<(unsigned)grid, 256, 0, s>>>(q, q_stride, scale, out, units, upr, nvec, cols);
-    GEO_CUDA_CHECK(cudaGetLastError());
-    return GEO_SC_OK;
+    return launch_behind(dequantize_int8_kernel<T, VEC, STEPS>, (unsigned)grid, 256, 0, s, 1, q, q_stride, scale, out, units, upr, nvec, cols);
 }
 
 template <typename T> int launch_dequantize(long long rows, int cols, const int8_t *q, long long q_stride, const float *scale, T *out, cudaStream_t s) {

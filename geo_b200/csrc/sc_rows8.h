@@ -157,6 +157,32 @@ template <typename T, int VEC> __device__ __forceinline__ void store_staged(uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 
+// These kernels are launched so that their CTAs may take their places while the kernel in front of them in the stream is
+// still finishing.  ahead_of_previous(): the kernel behind this one may do the same; after_previous(): from here on the
+// kernel in front has completed and its writes are visible.  Nothing in global memory is touched before that.
+__device__ __forceinline__ void ahead_of_previous() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
+// Launch of such a kernel, in clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t s, int cluster, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    GEO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return GEO_SC_OK;
+}
+
 inline bool dtype_known(int dtype) { return dtype == GEO_SC_DTYPE_F32 || dtype == GEO_SC_DTYPE_BF16 || dtype == GEO_SC_DTYPE_F16; }
 inline int dtype_size(int dtype) { return dtype == GEO_SC_DTYPE_F32 ? 4 : 2; }
 inline bool aligned_to(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }

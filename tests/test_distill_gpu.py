@@ -301,6 +301,45 @@ def test_captured_and_on_another_stream(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(captured, expect))
 
 
+def test_kernels_in_a_row_wait_for_each_other(cuda_device):
+    """Chains of all operators, one after the other into memory that is reused, against the same with the device waited for
+    after every call; eagerly and replayed."""
+    from geo_b200 import _lib
+    from geo_b200 import functional as F
+
+    g = torch.Generator().manual_seed(17)
+    cases = []
+    for m, n, k, dtype in ((1, 512, 2048, torch.bfloat16), (40, 1001, 513, torch.float32), (300, 10, 4096, torch.float16), (1500, 4096, 64, torch.float32),
+                           (3, 4096, 4096, torch.bfloat16), (700, 600, 1100, torch.float16)):
+        cases.append((torch.randn(m, k, generator=g).to(dtype).to(cuda_device), torch.randn(n, k, generator=g).to(cuda_device),
+                      torch.rand(k, generator=g).to(cuda_device), torch.randint(-1, n, (m, 8), generator=g).to(cuda_device),
+                      torch.randn(m, 8, generator=g).to(cuda_device)))
+
+    def chain(case, wait=lambda: None):
+        x, w, norm, indices, teacher = case
+        out = []
+        for step in (lambda: F.quantize_int8(w), lambda: F.rms_norm_int8(x, norm, residual=x),
+                     lambda: (F.linear_int8(*out[2:4], *out[:2]).requires_grad_(True),),
+                     lambda: (F.dequantize_int8(*out[2:4], x.dtype),),
+                     lambda: torch.autograd.grad(F.distillation_loss(out[5], indices, teacher, 2.0), out[5]),
+                     lambda: torch.autograd.grad(F.distillation_loss(out[5], indices, teacher, reduction="none").sum(), out[5])):
+            out.extend(step())
+            wait()
+        return [t.detach() for t in out]
+
+    expect = [chain(case, torch.cuda.synchronize) for case in cases]
+    for i in [0, 3, 1, 5, 2, 4] * 10:
+        assert all(torch.equal(a, b) for a, b in zip(chain(cases[i]), expect[i]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [chain(case) for case in cases]
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got, want in zip(captured, expect) for a, b in zip(got, want))
+    assert _lib.device_error_count() == 0
+
+
 @pytest.mark.parametrize("graph", [False, True])
 def test_training_against_a_fixed_point_teacher(cuda_device, graph):
     """A teacher on 8-bit integers (norm, linear layers) scores a batch, its top logits train the stochastic-computing
