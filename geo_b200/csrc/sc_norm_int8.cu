@@ -106,8 +106,9 @@ __device__ __forceinline__ RowStats join_stats(float ss, float top, int tpr, int
     RowStats r;
     r.top = warp_max_nan(top);
     r.ss = ss;
-    // infinite (or NaN) without a product that is, or vanished without being zero
-    r.again = NORM && r.top <= 3.402823466e38f && (!(ss <= 3.0e37f) || (ss < 1e-30f && r.top > 0.f));
+    // near the end of the range of 32 bits (32 warps add up) without a product that is infinite or NaN, or vanished without
+    // being zero
+    r.again = NORM && r.top <= 3.402823466e38f && (!(ss <= 1.0e37f) || (ss < 1e-30f && r.top > 0.f));
     if (tpr > 32) {
         if (lane == 0) {
             part_ss[turn][warp] = ss;

@@ -104,6 +104,18 @@ def test_norm_of_extreme_rows(cuda_device, dtype):
     assert (q == 0).all() and (scale == 0).all()
 
 
+@pytest.mark.parametrize("value", [1.7e17, 1.05e17, 6e16, 1e18, 3e-16, 1e-18, 3e-20])
+@pytest.mark.parametrize("cols", [16384, 16383, 40000, 300])
+def test_norm_at_the_ends_of_the_sum(cuda_device, value, cols):
+    """Rows whose squares fit 32 bits one by one and warp by warp, but not together, or nearly vanish."""
+    from geo_b200 import functional as F
+
+    x = torch.full((3, cols), value)
+    x[1, ::2] *= -0.5
+    w = torch.ones(cols)
+    check_norm(x.to(cuda_device), None, w, 0.0, F.rms_norm_int8(x.to(cuda_device), w.to(cuda_device), eps=0.0))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_norm_strides_and_shapes(cuda_device, dtype):
     from geo_b200 import functional as F
