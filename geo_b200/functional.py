@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from ._lib import rows as _rows
 from .guide import sc_conv2d_with_guide
 
 prec_default = 7  # 8-bit integers, one bit for the sign (utils_functional.py:28)
@@ -165,7 +166,8 @@ def sc_forward_counts(activation, weight, bit_length, forward="1d_bin", padding=
     return ops.sc_conv2d(activation, weight, bit_length, forward, (p1, p0), **kw)
 
 
-# ---- 8-bit integers with one scale per row: the fixed-point counterpart of the SC layers, for evaluation ----
+# ---- 8-bit integers with one scale per row: the fixed-point counterpart of the SC layers, for evaluation
+# (checks, allocation and launches in C++: the module that _lib.rows() loads) ----
 
 
 def rms_norm_int8(x, weight, residual=None, eps=1e-6):
@@ -176,25 +178,25 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     ``q * scale`` is the normalised row.  Returns ``(q, scale)``, or ``(q, scale, r)`` when a residual is given.
     ``x`` float32, bfloat16 or float16, any leading dimensions; ``weight`` of any of these types.  A row of zeros has
     scale 0; a row that holds an infinity or a NaN has q = 0 and scale = NaN.  Evaluation only, CUDA tensors only."""
-    return ops.rms_norm_int8(x, weight, residual, eps)
+    return _rows().rms_norm_int8(x, weight, residual, eps)
 
 
 def quantize_int8(x):
     """``(q, scale)`` with ``q = round(127 x / max|x|)`` and ``scale = max|x| / 127`` over the last dimension: tokens
     with a scale each, or a weight ``[out, in]`` with a scale per output channel.  Evaluation only."""
-    return ops.quantize_int8(x)
+    return _rows().quantize_int8(x)
 
 
 def dequantize_int8(q, scale, dtype=torch.float32):
     """The values ``q * scale`` that the integers of :func:`quantize_int8` and :func:`rms_norm_int8` stand for."""
-    return ops.dequantize_int8(q, scale, dtype)
+    return _rows().dequantize_int8(q, scale, dtype)
 
 
 def linear_int8(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32):
     """``(q @ weight_q.T) * scale[..., None] * weight_scale + bias`` for 8-bit integers ``q [..., k]`` with a scale per
     row and ``weight_q [n, k]`` with a scale per output channel: exact integer sums, one rounding to ``dtype``.
     ``k`` up to 131071.  Evaluation only."""
-    return ops.linear_int8(q, scale, weight_q, weight_scale, bias, dtype)
+    return _rows().linear_int8(q, scale, weight_q, weight_scale, bias, dtype)
 
 
 # ---- training against a teacher ---------------------------------------------------------------------------
@@ -214,4 +216,4 @@ def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=N
 
     ``scale`` is part of the loss; a loss scale or the loss's share in a sum is best given here, because the gradient
     is computed along with the loss for an upstream gradient of 1 and again where that turns out to be another."""
-    return ops.distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)
+    return _rows().distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)

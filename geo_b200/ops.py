@@ -480,33 +480,3 @@ def epilogue_backward(counts, in_bit_length, grad_out, weight, mean, invstd, wq,
             scratch.numel(), _stream_ptr(dev)), "geo_sc_epilogue_backward")
     STATS.launches += 3
     return gx, gw, gb
-
-
-# ---- 8-bit integers with one scale per row, and the distillation loss (checks and launches in C++: _lib.rows) ----
-
-
-def rms_norm_int8(x, weight, residual=None, eps=1e-6):
-    """Root-mean-square norm of the rows of ``x`` (plus ``residual``) as 8-bit integers -> (q, scale) or, with a
-    residual, (q, scale, x + residual); shapes [..., cols], [...], [..., cols]."""
-    return _lib.rows().rms_norm_int8(x, weight, residual, eps)
-
-
-def quantize_int8(x):
-    """Rows of ``x`` as 8-bit integers with one scale per row -> (q [..., cols], scale [...])."""
-    return _lib.rows().quantize_int8(x)
-
-
-def dequantize_int8(q, scale, dtype=torch.float32):
-    """``q * scale`` per row, rounded once to ``dtype``."""
-    return _lib.rows().dequantize_int8(q, scale, dtype)
-
-
-def linear_int8(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32):
-    """8-bit matrix product [..., k] x [n, k] -> [..., n] with a scale per row of either operand.  Operands whose rows
-    do not start on 16-byte boundaries are copied first (the quantisers of this module leave rows that do)."""
-    return _lib.rows().linear_int8(q, scale, weight_q, weight_scale, bias, dtype)
-
-
-def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=None, reduction="batchmean", scale=1.0):
-    """Distillation loss, differentiable in ``logits``: a scalar, or one value per row for ``reduction='none'``."""
-    return _lib.rows().distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)
