@@ -12,8 +12,9 @@
 // q_j = 2^(z_j c - r) / S.  The argument is one fused multiply-add, rounded relative to itself, so the terms which carry
 // the sum have small errors; that r is rounded does not matter, because every term and every partial sum is taken
 // against a reference that is kept as it is.  Past |m c| = 2^30 (rows masked by the type's lowest value throughout) that
-// rounding is too coarse; there two different values of any of the types are at least 64 apart in the exponent, and
-// logits other than m count as -inf, m as 0.
+// rounding is too coarse; there two different values of any of the types are at least 64 apart in the exponent, so that in
+// q logits other than m count as -inf, m as 0.  In the loss log q = (z - m) / T - log S is taken of the logit itself: it is
+// finite where q is not above 0.
 // Sums over the entries and over the rows are joined in a fixed order, the loss in 64 bits.
 //
 // What bounds it: HBM, one read of the logits and, with the gradient, one write.  A team copies its share of a row into
@@ -476,10 +477,11 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             if (STATS && GRAD && scribe) merge_entries(en, pr.top, from, to, psum);
             if (STATS && scribe && rank == 0) {
                 const double log_s = logf(sum), log_p = logf(psum);   // half a step of about 10 at most: what is added to them is exact
+                const double largest = flat ? (double)m * (double)c : (double)ref;   // what S is taken against
                 double loss = 0;
                 for (int k = lane; k < pr.top; k += 32)
                     if (en.idx[k] >= 0 && en.prob[k] > 0.f)
-                        loss += (double)(en.prob[k] / psum) * (((double)en.diff[k] - log_p) - (((double)seen(en.own[k]) * (double)c - (double)ref) * 0.6931471805599453 - log_s));
+                        loss += (double)(en.prob[k] / psum) * (((double)en.diff[k] - log_p) - (((double)en.own[k] * (double)c - largest) * 0.6931471805599453 - log_s));
                 loss = warp_sum(loss);
                 if (lane == 0) {
                     const double t = pr.temperature;

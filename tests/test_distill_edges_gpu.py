@@ -1,0 +1,56 @@
+"""Distillation loss: rows at the far end of the exponent, and gradients across the border of a captured graph."""
+import math
+
+import pytest
+import torch
+
+from test_distill_gpu import check, make
+
+pytestmark = pytest.mark.gpu
+
+
+def far_rows(dtype, vocab, T, device):
+    """Rows whose logits are past 2^30 in the exponent z log2(e) / T, with entries on logits that are not the largest."""
+    top = {1e-6: 1000.0, 5e-5: 60000.0, 1.0: 2e9}[T]
+    logits, indices, teacher = make(5, vocab, 4, dtype, vocab, device)
+    with torch.no_grad():
+        logits[0, :4] = torch.tensor([top, top * 0.75, 3.0, 4.0], device=device)
+        indices[0], teacher[0] = torch.tensor([0, 1, -1, -1], device=device), 0.0
+        logits[1] = -top                      # the largest is negative, and twice there
+        logits[1, 2:4] = -top * 0.8
+        indices[1], teacher[1] = torch.tensor([3, 1, vocab - 1, 2], device=device), 0.5
+        logits[2, vocab - 1] = top            # one entry, and it is not the largest logit
+        indices[2] = torch.tensor([0, -1, -1, -1], device=device)
+        logits[3, 1] = top
+        logits[3, 2] = -math.inf              # an entry that the student rules out, without a share
+        indices[3], teacher[3] = torch.tensor([1, 2, 0, 0], device=device), torch.tensor([0.0, -math.inf, 1.0, 1.0], device=device)
+    return logits, indices, teacher
+
+
+FAR = [(torch.float32, 1e-6), (torch.float32, 1.0), (torch.bfloat16, 1e-6), (torch.bfloat16, 1.0), (torch.float16, 1e-6), (torch.float16, 5e-5)]
+
+
+@pytest.mark.parametrize("dtype, T", FAR)
+@pytest.mark.parametrize("vocab", [5, 41, 3000, 90001, 300001])
+def test_entries_below_the_largest_logit_far_out(cuda_device, dtype, T, vocab):
+    """The loss of an entry that is not the row's largest logit is finite, however far its probability lies below the range."""
+    logits, indices, teacher = far_rows(dtype, vocab, T, cuda_device)
+    loss, _ = check(logits, indices, teacher, T)
+    assert loss.isfinite().all() and (loss[:3] > 0).all()
+    check(logits, indices, teacher, T, up=torch.tensor([1.0, -2.0, 0.5, 1.0, 3.0], device=cuda_device))
+    check(logits, indices, teacher, T, reduction="batchmean")
+    check(logits, indices, teacher, T, reduction="sum", up=torch.tensor(-3.0, device=cuda_device))
+
+
+def test_far_rows_by_hand(cuda_device):
+    from geo_b200 import functional as F
+
+    entries, equal = torch.tensor([[0, 1]], device=cuda_device), torch.zeros(1, 2, device=cuda_device)
+    loss = F.distillation_loss(torch.tensor([[1000.0, 999.0, 3.0, 4.0]], device=cuda_device), entries, equal, 1e-6)
+    # p = 1/2 twice, log q = 0 and -1e6: T^2 (log(1/2) + 1e6 / 2)
+    assert abs(float(loss) - 1e-12 * (5e5 - math.log(2))) <= 5e-7 * 2.0 ** -20
+    loss = F.distillation_loss(torch.tensor([[2e9, 1e9, 0.0, 1.0]], device=cuda_device), entries, equal)
+    assert abs(float(loss) - 5e8) <= 5e8 * 2.0 ** -20
+    # a student that rules the second entry out
+    loss = F.distillation_loss(torch.tensor([[2e9, -math.inf, 0.0, 1.0]], device=cuda_device), entries, equal)
+    assert float(loss) == math.inf
