@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         }
 
         float m = 0.f, sum = 0.f;
-        bool flat = false;   // m c out of range: a logit is either m or nothing
-        auto seen = [&](float v) { return !flat ? v : v == m ? 0.f : NEG_INF; };
+        bool flat = false;   // m c out of range: a logit is either m or nothing, or NaN
+        auto seen = [&](float v) { return !flat ? v : v < m ? NEG_INF : v - m; };   // a NaN stays one
         auto out_of_range = [&]() { return fabsf(m) <= 3.402823466e38f && !(fabsf(scaled(m)) <= FAR); };
         // Largest logit and sum of the warp.  A thread's reference is the first largest value that it meets, and moves only
         // for one that is 2^32 times as probable (some lane would move it at nearly every vector otherwise); sums stay far

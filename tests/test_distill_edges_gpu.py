@@ -54,3 +54,20 @@ def test_far_rows_by_hand(cuda_device):
     # a student that rules the second entry out
     loss = F.distillation_loss(torch.tensor([[2e9, -math.inf, 0.0, 1.0]], device=cuda_device), entries, equal)
     assert float(loss) == math.inf
+
+
+@pytest.mark.parametrize("dtype, T", FAR)
+@pytest.mark.parametrize("vocab", [41, 3000, 90001, 300001])
+def test_nan_among_far_rows(cuda_device, dtype, T, vocab):
+    """A NaN logit makes its row's loss and gradient NaN, as it does in every other row."""
+    from geo_b200 import functional as F
+
+    logits, indices, teacher = far_rows(dtype, vocab, T, cuda_device)
+    with torch.no_grad():
+        logits[0, vocab - 2] = math.nan      # no entry
+        logits[1, 3] = math.nan              # an entry
+    for reduction, up in (("none", torch.ones(5, device=cuda_device)), ("batchmean", None)):
+        loss = F.distillation_loss(logits, indices, teacher, T, reduction=reduction)
+        (grad,) = torch.autograd.grad(loss, logits, up)
+        assert grad[:2].isnan().all() and grad[2:].isfinite().all()
+        assert loss.isnan().tolist() == ([True, True, False, False, False] if reduction == "none" else True)
