@@ -20,14 +20,14 @@ namespace {
 
 // 16 bytes of a row from byte `at` on, zeros from byte k on.
 __device__ __forceinline__ uint4 load16(const int8_t *row, int at, int k) {
-    if (at + 16 <= k) return __ldg((const uint4 *)(row + at));
+    if (at + 16 <= k) return *(const uint4 *)(row + at);
     uint32_t v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int b = at + 4 * i;
         v[i] = 0;
         if (b + 4 <= k) {
-            v[i] = __ldg((const uint32_t *)(row + b));
+            v[i] = *(const uint32_t *)(row + b);
         } else if (b < k) {
             v[i] = (uint8_t)row[b];
             if (b + 1 < k) v[i] |= (uint32_t)(uint8_t)row[b + 1] << 8;
@@ -80,14 +80,14 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
         uint4 a[UNROLL], b[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            a[u] = __ldg((const uint4 *)(wa + kc + chunk(u)));
-            b[u] = __ldg((const uint4 *)(wb + kc + chunk(u)));
+            a[u] = *(const uint4 *)(wa + kc + chunk(u));
+            b[u] = *(const uint4 *)(wb + kc + chunk(u));
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             uint4 x[NT];
 #pragma unroll
-            for (int j = 0; j < NT; j++) x[j] = __ldg((const uint4 *)(xr[j] + kc + chunk(u)));
+            for (int j = 0; j < NT; j++) x[j] = *(const uint4 *)(xr[j] + kc + chunk(u));
             step(a[u], b[u], x);
         }
     }

@@ -277,10 +277,10 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         float xs[XS], ws = 0.f, b = 0.f;
         auto ask_scales = [&](int t) {
             const int n0 = (t % ntiles_n) * 128 * CTAS + rank * 128 + quarter * 32 + lane, m0 = (t / ntiles_n) * BN + half * COLS;
-            ws = t < ntiles && n0 < pr.n ? __ldg(pr.w_scale + n0) : 0.f;
-            b = t < ntiles && pr.bias && n0 < pr.n ? __ldg(pr.bias + n0) : 0.f;
+            ws = t < ntiles && n0 < pr.n ? pr.w_scale[n0] : 0.f;
+            b = t < ntiles && pr.bias && n0 < pr.n ? pr.bias[n0] : 0.f;
 #pragma unroll
-            for (int i = 0; i < XS; i++) xs[i] = t < ntiles && i * 32 + lane < COLS && m0 + i * 32 + lane < pr.m ? __ldg(pr.x_scale + m0 + i * 32 + lane) : 0.f;
+            for (int i = 0; i < XS; i++) xs[i] = t < ntiles && i * 32 + lane < COLS && m0 + i * 32 + lane < pr.m ? pr.x_scale[m0 + i * 32 + lane] : 0.f;
         };
         ask_scales(worker);
         if (SPLIT) {   // for the whole CTA, which shares out the columns

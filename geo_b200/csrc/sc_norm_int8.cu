@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(256) dequantize_int8_kernel(const int8_t *q, l
 #pragma unroll
     for (int j = 0; j < STEPS; j++)
         if (first + j * 32 < nvec) v[j] = load_pack<int8_t, VEC>(q + (long long)(first + j * 32) * VEC);
-    const float s = __ldg(scale + row);
+    const float s = scale[row];
 #pragma unroll
     for (int j = 0; j < STEPS; j++)
         if (first + j * 32 < nvec) {

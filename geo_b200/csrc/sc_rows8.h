@@ -159,7 +159,9 @@ template <typename T, int VEC> __device__ __forceinline__ void store_staged(uint
 
 // These kernels are launched so that their CTAs may take their places while the kernel in front of them in the stream is
 // still finishing.  ahead_of_previous(): the kernel behind this one may do the same; after_previous(): from here on the
-// kernel in front has completed and its writes are visible.  Nothing in global memory is touched before that.
+// kernel in front has completed and its writes are visible.  Nothing in global memory is touched before that, and nothing
+// is read through the read-only path (__ldg, ld.global.nc, const __restrict__): that is promised only for memory that
+// nobody writes while the kernel lives, and the kernel in front writes its results while this one waits.
 __device__ __forceinline__ void ahead_of_previous() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
