@@ -292,7 +292,8 @@ class Linear_Int8(nn.Module):
     """Linear layer on 8-bit integers, for evaluation: weights with a scale per output channel, laid out once when the
     layer is made, inputs with a scale per row (:func:`geo_b200.functional.linear_int8`).  The fixed-point counterpart
     of :class:`Linear_Or`.  ``forward`` takes floating-point rows (quantised here) or the pair ``(q, scale)`` of
-    :class:`RMSNorm_Int8`; the output has the input's dtype, that of ``dtype`` for a pair (default float32)."""
+    :class:`RMSNorm_Int8`; the output has the input's dtype, that of ``dtype`` for a pair (default float32).
+    ``weight_scale`` and ``bias`` are float32 and stay so when the model that holds the layer is cast."""
 
     def __init__(self, in_features, out_features, bias=True):
         super().__init__()
@@ -301,6 +302,15 @@ class Linear_Int8(nn.Module):
         self.register_buffer("weight_q", torch.zeros(self.out_features, (self.in_features + 15) // 16 * 16, dtype=torch.int8))
         self.register_buffer("weight_scale", torch.zeros(self.out_features))
         self.register_buffer("bias", torch.zeros(self.out_features) if bias else None)
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = {name: getattr(self, name) for name in ("weight_scale", "bias")}
+        super()._apply(fn, *args, **kwargs)
+        for name, before in kept.items():   # casts (half(), bfloat16(), to(dtype)) only move these
+            now = getattr(self, name)
+            if now is not None and now.dtype != torch.float32:
+                setattr(self, name, before.to(now.device, torch.float32))
+        return self
 
     @classmethod
     def from_float(cls, linear):

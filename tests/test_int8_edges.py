@@ -24,3 +24,20 @@ def test_kernels_launched_ahead_read_by_plain_loads():
             ahead.append(name)
             assert not re.search(r"\b__ldg\b|ld\.global\.nc|\b__restrict__\b", code), name
     assert {"sc_norm_int8.cu", "sc_linear_int8.cu", "sc_linear_int8_tc.cu", "sc_distill.cu"} <= set(ahead)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.float16), lambda m: m.double(),
+                                  lambda m: torch.nn.Sequential(m).to(torch.bfloat16)[0]])
+def test_cast_layers_keep_their_scales(cast):
+    """Scales and bias of the 8-bit layer are part of its arithmetic, not of the model's element type."""
+    layer = layers.Linear_Int8(17, 5)
+    layer.weight_scale.copy_(torch.rand(5) + 1 / 3)
+    layer.bias.copy_(torch.rand(5) + 1 / 3)
+    scale, bias = layer.weight_scale.clone(), layer.bias.clone()
+    layer = cast(layer)
+    assert layer.weight_q.dtype == torch.int8
+    assert torch.equal(layer.weight_scale, scale) and torch.equal(layer.bias, bias)
+    assert set(layer.state_dict()) == {"weight_q", "weight_scale", "bias"}
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):     # refused for the device, not for a type
+        layer((i8(2, 17), torch.ones(2)))
+    assert cast(layers.Linear_Int8(17, 5, bias=False)).bias is None
