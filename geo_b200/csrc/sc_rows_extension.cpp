@@ -5,6 +5,7 @@
 //
 // Arguments are checked before the device is looked at, so that a wrong shape is named on a machine without a GPU too.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -65,9 +66,13 @@ void one_device(std::initializer_list<const Tensor *> tensors) {
 }
 
 void evaluation_only(const char *name, std::initializer_list<const Tensor *> tensors) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor *t : tensors)
-        TORCH_CHECK(!t || !t->requires_grad(), name, " has no gradient (evaluation only): call it under torch.no_grad() or detach its inputs");
+    // a gradient is asked for under grad mode only, a tangent (forward mode) whatever that is
+    const bool grad = at::GradMode::is_enabled(), tangent = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor *t : tensors) {
+        if (!t) continue;
+        TORCH_CHECK(!grad || !t->requires_grad(), name, " has no gradient (evaluation only): call it under torch.no_grad() or detach its inputs");
+        TORCH_CHECK(!tangent || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative (evaluation only): give it the primal values");
+    }
 }
 
 const Tensor *ptr(const OptTensor &t) { return t.has_value() && t->defined() ? &*t : nullptr; }

@@ -71,3 +71,18 @@ def test_nan_among_far_rows(cuda_device, dtype, T, vocab):
         (grad,) = torch.autograd.grad(loss, logits, up)
         assert grad[:2].isnan().all() and grad[2:].isfinite().all()
         assert loss.isnan().tolist() == ([True, True, False, False, False] if reduction == "none" else True)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", ["logits", "teacher", "weight"])
+def test_tangents_are_refused(cuda_device, which, grad):
+    import torch.autograd.forward_ad as ad
+
+    from geo_b200 import functional as F
+
+    logits, indices, teacher = make(4, 20, 3, torch.float32, 1, cuda_device)
+    given = {"logits": logits.detach(), "teacher": teacher, "weight": torch.ones(4, device=cuda_device)}
+    with ad.dual_level(), torch.set_grad_enabled(grad):
+        given[which] = ad.make_dual(given[which], torch.ones_like(given[which]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            F.distillation_loss(given["logits"], indices, given["teacher"], weight=given["weight"])

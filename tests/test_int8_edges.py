@@ -41,3 +41,23 @@ def test_cast_layers_keep_their_scales(cast):
     with pytest.raises(RuntimeError, match="CUDA tensors only"):     # refused for the device, not for a type
         layer((i8(2, 17), torch.ones(2)))
     assert cast(layers.Linear_Int8(17, 5, bias=False)).bias is None
+
+
+@pytest.mark.parametrize("call", [
+    lambda dual: F.rms_norm_int8(dual(2, 8), torch.ones(8)),
+    lambda dual: F.rms_norm_int8(torch.zeros(2, 8), dual(8)),
+    lambda dual: F.rms_norm_int8(torch.zeros(2, 8), torch.ones(8), residual=dual(2, 8)),
+    lambda dual: F.quantize_int8(dual(2, 8)),
+    lambda dual: F.dequantize_int8(i8(2, 8), dual(2)),
+    lambda dual: F.linear_int8(i8(2, 8), dual(2), i8(3, 8), torch.ones(3)),
+    lambda dual: F.linear_int8(i8(2, 8), torch.ones(2), i8(3, 8), dual(3)),
+    lambda dual: F.linear_int8(i8(2, 8), torch.ones(2), i8(3, 8), torch.ones(3), bias=dual(3)),
+])
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(call, grad):
+    """Forward-mode derivatives are not dropped without a word, under no_grad (which does not concern them) neither."""
+    import torch.autograd.forward_ad as ad
+
+    with ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(RuntimeError, match="evaluation only"):
+            call(lambda *shape: ad.make_dual(torch.ones(*shape), torch.ones(*shape)))
