@@ -6,6 +6,7 @@
 // Arguments are checked before the device is looked at, so that a wrong shape is named on a machine without a GPU too.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -209,9 +210,19 @@ Tensor linear_int8(const Tensor &q, const Tensor &scale, const Tensor &weight_q,
     return out;
 }
 
+// The graph capture that the current stream is part of; 0: none.
+int64_t capture_id() {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream().stream(), &status, &id));
+    return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 // The loss with its gradient.  With a scalar loss the forward pass writes the gradient for an upstream gradient of 1
 // along with the loss, so that the logits are read once; the backward pass hands that over, writing it anew (decided on
-// the device) where the upstream gradient is another.  A second backward pass over the same graph writes its own.
+// the device) where the upstream gradient is another.  A second backward pass over the same graph writes its own, and so
+// does one on the other side of a graph capture: replayed without the forward pass, it would find what an earlier replay
+// or the gradient's owner has left in that memory.
 struct Distillation : torch::autograd::Function<Distillation> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const Tensor &indices, const Tensor &teacher,
                           const OptTensor &weight_, double temperature, double scale, bool mean, bool need) {
@@ -237,7 +248,10 @@ struct Distillation : torch::autograd::Function<Distillation> {
             ctx->saved_data["temperature"] = temperature;
             ctx->saved_data["scale"] = scale;
             ctx->saved_data["mean"] = mean;
-            if (grad.defined()) ctx->saved_data["ready"] = grad;
+            if (grad.defined()) {
+                ctx->saved_data["ready"] = grad;
+                ctx->saved_data["capture"] = capture_id();
+            }
         }
         return mean ? loss : row_loss;
     }
@@ -253,7 +267,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
             const Tensor z = rows_of(logits), up = upstream[0].to(at::kFloat).contiguous();
             bool ready = false;
             const auto it = ctx->saved_data.find("ready");
-            if (it != ctx->saved_data.end()) {
+            if (it != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_id()) {
                 grad = it->second.toTensor();
                 ctx->saved_data.erase(it);
                 ready = true;

@@ -86,3 +86,31 @@ def test_tangents_are_refused(cuda_device, which, grad):
         given[which] = ad.make_dual(given[which], torch.ones_like(given[which]))
         with pytest.raises((RuntimeError, NotImplementedError)):
             F.distillation_loss(given["logits"], indices, given["teacher"], weight=given["weight"])
+
+
+def test_backward_captured_after_an_eager_forward(cuda_device):
+    """The gradient that an eager forward pass has written is not what a captured backward pass hands over: the graph
+    writes its own at every replay, whatever the upstream gradient was before or was done with the last one's memory."""
+    from geo_b200 import functional as F
+
+    source, indices, teacher = make(7, 3001, 12, torch.float32, 5, cuda_device)
+    expect = torch.autograd.grad(F.distillation_loss(source, indices, teacher, 2.0), source)[0]
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        logits = source.detach().clone().requires_grad_(True)
+        up = torch.ones((), device=cuda_device)
+        loss = F.distillation_loss(logits, indices, teacher, 2.0)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            (grad,) = torch.autograd.grad(loss, logits, up, retain_graph=True)
+        for factor in (2.0, 1.0, -1.0, 1.0):
+            up.fill_(factor)
+            graph.replay()
+            assert torch.equal(grad, expect * factor)
+        grad.zero_()
+        graph.replay()
+        assert torch.equal(grad, expect)
+        # the eager pass's own gradient is still to be had
+        assert torch.equal(torch.autograd.grad(loss, logits, up)[0], expect)
+    torch.cuda.current_stream().wait_stream(stream)
