@@ -71,6 +71,8 @@ class TrainStep:
             self._capture(inputs, targets, teacher)
         sx, sy, steacher, sloss, sout = self._static
         if steacher is not None:
+            if len(teacher) != len(steacher):
+                raise ValueError(f"graph=True: the teacher had {len(steacher)} tensors at capture, now {len(teacher)}")
             for static, now in zip(steacher, teacher):
                 if static.shape != now.shape or static.dtype != now.dtype:
                     raise ValueError(f"graph=True: the teacher's entries were {static.dtype} {tuple(static.shape)} at capture, "

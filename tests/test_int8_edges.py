@@ -61,3 +61,17 @@ def test_tangents_are_refused(call, grad):
     with ad.dual_level(), torch.set_grad_enabled(grad):
         with pytest.raises(RuntimeError, match="evaluation only"):
             call(lambda *shape: ad.make_dual(torch.ones(*shape), torch.ones(*shape)))
+
+
+def test_replayed_step_refuses_a_teacher_of_another_form():
+    """A captured step copies the teacher's entries into its own: what does not correspond is named, not left out."""
+    class Replay:
+        def replay(self):
+            raise AssertionError("replayed")
+
+    step = train.TrainStep(torch.nn.Linear(4, 4), graph=True, distillation=layers.DistillationLoss())
+    entries = (torch.zeros(2, 3).long(), torch.zeros(2, 3), torch.ones(2))      # with a weight per row
+    step._graph, step._static = Replay(), (torch.zeros(2, 4), torch.zeros(2).long(), entries, None, None)
+    for teacher in (entries[:2], entries[:1], (*entries, torch.ones(2))):
+        with pytest.raises(ValueError):
+            step(torch.zeros(2, 4), torch.zeros(2).long(), teacher=teacher)
