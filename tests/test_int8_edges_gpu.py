@@ -21,3 +21,27 @@ def test_layers_of_a_cast_model(cuda_device, dtype):
         expect = model(x)
         assert torch.equal(model.to(dtype)(x), expect)
         assert torch.equal(model.cpu().to(cuda_device)(x), expect)
+
+
+# Error of a row's scale, whatever its length: a thread adds at most 32 rounded products one after the other, what lies
+# past those in parts of at most 16 products which are joined in 64 bits (one rounding back, one addition), five shuffles
+# join a warp and five the warps: 32 + 2 + 10 half steps of the sum, halved by the root; the mean's division and the
+# addition of eps, halved as well, the root, and two divisions.
+SCALE_ERROR = (44 / 2 + 2 / 2 + 3) * STEP32
+
+
+@pytest.mark.parametrize("cols", [40000, 60001, (1 << 20) - 4, (1 << 26) - 4, (1 << 26) - 1])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_error_of_the_scale_does_not_grow_with_the_row(cuda_device, cols, with_residual):
+    """Squares of 1 + 2^-9: a sum of many in 32 bits loses the 2^-9 of each as soon as it is large."""
+    from geo_b200 import functional as F
+
+    value = (1 + 2.0 ** -9) ** 0.5
+    x = torch.full((1, cols), value, device=cuda_device)
+    x[0, 7] = 3.0
+    res = torch.zeros(1, cols, device=cuda_device) if with_residual else None
+    q, scale = F.rms_norm_int8(x, torch.ones(cols, device=cuda_device), res, eps=0.0)[:2]
+    single = float(x[0, 0])
+    expect = 3 / 127 / (((cols - 1) * single * single + 9) / cols) ** 0.5
+    assert abs(float(scale) - expect) <= SCALE_ERROR * expect
+    assert q[0, 7] == 127 and (q[0, 8:] == round(127 * single / 3)).all()
