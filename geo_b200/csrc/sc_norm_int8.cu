@@ -129,7 +129,9 @@ template <bool NORM> __device__ __forceinline__ float row_scale(const RowStats &
     if (!(st.top <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
     if (!NORM || st.top == 0.f) return st.top / 127.f;
     if (st.again) return (float)((double)st.top / 127.0 / sqrt(total / cols + (double)eps));
-    return st.top / sqrtf(st.ss / (float)cols + eps) / 127.f;
+    const float rms = sqrtf(st.ss / (float)cols + eps);
+    const float largest = st.top / rms;   // of the normalised row: may leave the range where its 127th part does not
+    return largest <= 3.402823466e38f ? largest / 127.f : st.top / 127.f / rms;
 }
 
 // Joins the 64-bit sums of a row (every thread of the CTA takes part).

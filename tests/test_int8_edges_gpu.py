@@ -45,3 +45,21 @@ def test_error_of_the_scale_does_not_grow_with_the_row(cuda_device, cols, with_r
     expect = 3 / 127 / (((cols - 1) * single * single + 9) / cols) ** 0.5
     assert abs(float(scale) - expect) <= SCALE_ERROR * expect
     assert q[0, 7] == 127 and (q[0, 8:] == round(127 * single / 3)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("unit", [1.0, 2.0 ** -14, 2.0 ** -45])
+@pytest.mark.parametrize("cols", [4, 5, 64, 1000, 4096])
+def test_scale_near_the_end_of_its_range(cuda_device, dtype, cols, unit):
+    """A weight so large that max|p| / rms leaves the range of 32 bits although the scale, 1/127 of it, does not."""
+    from geo_b200 import functional as F
+
+    x = torch.zeros(3, cols, dtype=dtype, device=cuda_device)
+    x[0, 0], x[1, cols - 1], x[2, 1] = unit, -0.5 * unit, 0.75 * unit
+    x[2, 2] = 0.25 * unit
+    if dtype == torch.float16 and unit < 2.0 ** -14:
+        x[:, 0] = 2.0 ** -24         # the type's smallest value
+    w = torch.full((cols,), 3e38, device=cuda_device)
+    q, scale = F.rms_norm_int8(x, w, eps=0.0)
+    assert scale.isfinite().all()
+    check_norm(x, None, w, 0.0, (q, scale))
