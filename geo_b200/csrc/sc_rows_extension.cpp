@@ -311,12 +311,12 @@ Tensor distillation_loss(const Tensor &logits, const Tensor &indices, const Tens
     if (weight && (weight->sizes() != rows || weight->scalar_type() != at::kFloat))
         REFUSE_VALUE("weight must be float32 of shape ", rows, ", got ", weight->scalar_type(), weight->sizes());
     if (!(temperature >= 1e-6 && temperature <= 1e6)) REFUSE_VALUE("temperature must lie in [1e-6, 1e6], got ", temperature);
-    if (!(std::abs(scale) < 3.4e38)) REFUSE_VALUE("scale must be finite, got ", scale);
+    if (reduction == "sum") scale *= std::max<int64_t>(1, logits.numel() / logits.size(-1));   // the kernels divide by the rows
+    if (!(std::abs(scale) < 3.4e38)) REFUSE_VALUE("scale (for a sum, times the number of rows) must be finite in 32 bits, got ", scale);
     const bool grad_mode = at::GradMode::is_enabled();
     if (grad_mode && (teacher.requires_grad() || (weight && weight->requires_grad())))
         REFUSE_VALUE("distillation_loss has no gradient for teacher_logits and weight: detach them");
     one_device({&logits, &indices, &teacher, weight});
-    if (reduction == "sum") scale *= std::max<int64_t>(1, logits.numel() / logits.size(-1));   // the kernels divide by the rows
     return Distillation::apply(logits, indices.contiguous(), teacher.contiguous(), weight ? OptTensor(weight->contiguous()) : OptTensor(), temperature, scale,
                                reduction != "none", grad_mode && logits.requires_grad());
 }

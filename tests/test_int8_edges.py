@@ -75,3 +75,12 @@ def test_replayed_step_refuses_a_teacher_of_another_form():
     for teacher in (entries[:2], entries[:1], (*entries, torch.ones(2))):
         with pytest.raises(ValueError):
             step(torch.zeros(2, 4), torch.zeros(2).long(), teacher=teacher)
+
+
+def test_scale_of_a_sum_that_leaves_the_range_is_refused():
+    """The kernels take the scale times the number of rows; past 32 bits the loss would be infinite."""
+    entries = torch.zeros(4096, 1).long(), torch.zeros(4096, 1)
+    with pytest.raises(ValueError):
+        F.distillation_loss(torch.zeros(4096, 8), *entries, reduction="sum", scale=1e36)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        F.distillation_loss(torch.zeros(4096, 8), *entries, reduction="batchmean", scale=1e36)
