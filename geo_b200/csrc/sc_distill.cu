@@ -51,8 +51,7 @@ struct DistillParams {
     int vocab, top, index64, teacher_dtype;
     int upstream_rows;   // upstream has one value per row (else one value)
     int skip_one;        // rows whose upstream is 1 keep the gradient that the forward pass has written
-    float temperature, scale;
-    float loss_factor, grad_factor;
+    float temperature, loss_factor, grad_factor;
 };
 
 __device__ __forceinline__ float ex2(float x) {

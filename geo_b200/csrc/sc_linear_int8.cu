@@ -10,7 +10,7 @@
 // linear_int8_mma_kernel: `mma.sync.m16n8k32` with the weights as the 16-row operand, read once from memory straight
 // into fragments.  The order of k inside a product is free, so a lane takes 16 consecutive bytes of its weight row and
 // the same 16 bytes of its token rows for two instructions: whole 16-byte loads, no shared memory, no shuffles.  A CTA
-// of eight warps owns 16 channels x 8 * NT tokens; the warps split k and join their integer sums in shared memory.
+// of eight warps owns 16 channels and all tokens; the warps split k and join their integer sums in shared memory.
 // Bound by the weights' bytes: 1 x 8192 x 8192 15.4 us (4.4 TB/s with the launch), 16 x 4096 x 4096 4.7 us.  Above 32
 // tokens the other kernel takes less (64 x 4096 x 4096: 7.9 us; 32 tokens: 6.6 here, 6.9 there).
 #include "sc_linear_int8.h"
@@ -51,8 +51,7 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
     ahead_of_previous();
     after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int mtiles = (p.m + NT * 8 - 1) / (NT * 8);
-    const int m0 = (int)(blockIdx.x % mtiles) * NT * 8, n0 = (int)(blockIdx.x / mtiles) * 16;
+    const int n0 = (int)blockIdx.x * 16;
     // rows past the end repeat the last one; their sums are not stored
     const int8_t *wa = p.w + (long long)min(n0 + g, p.n - 1) * p.w_stride;
     const int8_t *wb = p.w + (long long)min(n0 + g + 8, p.n - 1) * p.w_stride;
@@ -60,7 +59,7 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
     int acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        xr[j] = p.x + (long long)min(m0 + j * 8 + g, p.m - 1) * p.x_stride;
+        xr[j] = p.x + (long long)min(j * 8 + g, p.m - 1) * p.x_stride;
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[j][i] = 0;
     }
@@ -110,11 +109,11 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
     }
     __syncthreads();
     for (int i = threadIdx.x; i < NT * 8 * 16; i += blockDim.x) {
-        const int mi = i >> 4, ni = i & 15, m = m0 + mi, n = n0 + ni;
+        const int m = i >> 4, ni = i & 15, n = n0 + ni;
         if (m >= p.m || n >= p.n) continue;
         int s = 0;
 #pragma unroll
-        for (int w = 0; w < MMA_WARPS; w++) s += sums[w][mi][ni];
+        for (int w = 0; w < MMA_WARPS; w++) s += sums[w][m][ni];
         float v = (float)s * p.x_scale[m] * p.w_scale[n];
         if (p.bias) v += p.bias[n];
         ((T *)p.out)[m * p.out_stride + n] = from_float<T>(v);
@@ -122,11 +121,9 @@ __global__ void __launch_bounds__(32 * MMA_WARPS) linear_int8_mma_kernel(LinearP
 }
 
 template <typename T> int launch_mma(const LinearParams &p, cudaStream_t s) {
-    const int nt = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
-    const long long grid = (long long)((p.m + nt * 8 - 1) / (nt * 8)) * ((p.n + 15) / 16);
-    if (grid > 0x7fffffffLL) return fail(GEO_SC_ERR_TOO_LARGE, "%d tokens x %d channels", p.m, p.n);
+    const int nt = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;   // 8 * nt tokens hold all m
     const auto kernel = nt == 1 ? linear_int8_mma_kernel<T, 1> : nt == 2 ? linear_int8_mma_kernel<T, 2> : linear_int8_mma_kernel<T, 4>;
-    return launch_behind(kernel, (unsigned)grid, 32 * MMA_WARPS, 0, s, 1, p);
+    return launch_behind(kernel, (unsigned)((p.n + 15) / 16), 32 * MMA_WARPS, 0, s, 1, p);
 }
 
 }  // namespace

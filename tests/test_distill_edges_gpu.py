@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_distill_gpu import check, make
+from test_distill_gpu import check, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,38 @@ def test_backward_captured_after_an_eager_forward(cuda_device):
         # the eager pass's own gradient is still to be had
         assert torch.equal(torch.autograd.grad(loss, logits, up)[0], expect)
     torch.cuda.current_stream().wait_stream(stream)
+
+
+@pytest.mark.parametrize("vocab, top", [(10, 3), (10, 9), (3000, 12), (40000, 40)])
+def test_c_entry_points_row_by_row(cuda_device, vocab, top):
+    """What the C ABI offers beside the front end's calls: the gradient with a loss per row, and a backward pass over it that
+    leaves the rows alone whose upstream gradient is 1."""
+    import ctypes
+
+    from geo_b200 import _lib
+
+    L, rows, T = _lib.lib(), 9, 2.0
+    logits, indices, teacher = make(rows, vocab, top, torch.float32, 4, cuda_device)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    loss, stats = torch.empty(rows, device=cuda_device), torch.empty(rows, 2, device=cuda_device)
+    grad = torch.empty(rows, vocab, device=cuda_device)
+    _lib.check(L.geo_sc_distill_forward(rows, vocab, top, 0, logits.data_ptr(), vocab, indices.data_ptr(), 64, teacher.data_ptr(), 0, None, T, 1.5, 0,
+                                        loss.data_ptr(), stats.data_ptr(), None, grad.data_ptr(), stream), "geo_sc_distill_forward")
+    row, expect, row_bound, bound = reference(logits, indices, teacher, T, None, 1.5, torch.ones(rows))
+    assert ((loss.cpu().double() - row).abs() <= row_bound).all() and ((grad.cpu().double() - expect).abs() <= bound).all()
+    up = torch.tensor([1.0, 2.0, 1.0, -1.0, 0.0, 1.0, 1.0, 0.5, 1.0], device=cuda_device)
+    grad[up == 1] = -7.0     # not to be touched
+    _lib.check(L.geo_sc_distill_backward(rows, vocab, top, 0, logits.data_ptr(), vocab, indices.data_ptr(), 64, teacher.data_ptr(), 0, None, T, 1.5, 0,
+                                         stats.data_ptr(), up.data_ptr(), 1, grad.data_ptr(), stream), "geo_sc_distill_backward")
+    _, expect, _, bound = reference(logits, indices, teacher, T, None, 1.5, up)
+    assert (grad[up == 1] == -7).all()
+    rest = (up != 1).cpu()
+    assert ((grad.cpu().double() - expect).abs() <= bound)[rest].all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_backward_walks_over_many_small_rows(cuda_device, dtype):
+    """More rows than are resident in a pass that may have nothing to do."""
+    logits, indices, teacher = make(20000, 10, 4, dtype, 6, cuda_device)
+    check(logits, indices, teacher, 2.0, reduction="batchmean", up=torch.tensor(2.5, device=cuda_device))
+    check(logits, indices, teacher, 2.0, reduction="batchmean")

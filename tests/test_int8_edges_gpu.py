@@ -63,3 +63,23 @@ def test_scale_near_the_end_of_its_range(cuda_device, dtype, cols, unit):
     q, scale = F.rms_norm_int8(x, w, eps=0.0)
     assert scale.isfinite().all()
     check_norm(x, None, w, 0.0, (q, scale))
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_layer_from_a_stochastic_layer(cuda_device, bias):
+    """The integers of a Linear_Or are those of its full-precision weight, not of the one that its last forward has quantised."""
+    from geo_b200 import functional as F
+    from geo_b200 import layers
+
+    torch.manual_seed(3)
+    sc = layers.Linear_Or(32, 12, bias=bias).to(cuda_device)
+    kept = sc.weight_org.clone()
+    sc(torch.rand(4, 32, device=cuda_device))
+    assert not torch.equal(sc.weight, kept)
+    with torch.no_grad():
+        layer = layers.Linear_Int8.from_float(sc)
+        q, scale = F.quantize_int8(kept)
+        assert torch.equal(layer.weight_q[:, :32], q) and torch.equal(layer.weight_scale, scale)
+        x = torch.randn(5, 32, device=cuda_device)
+        xq, xs = F.quantize_int8(x)
+        assert torch.equal(layer(x), F.linear_int8(xq, xs, q, scale, sc.bias))
