@@ -415,8 +415,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         const float ref = flat ? 0.f : scaled(m), inv_s = 1.f / sum, a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, a_s = a * inv_s;
         const bool wide = GRAD && ((uintptr_t)(grad + sl.head) & 15) == 0;
         auto give_all = [&]() {   // the gradient apart from the teacher's share
-            if (!wide) {   // the rows of the gradient lie otherwise in memory than those of the logits
-                for (int j = from + tid; j < to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
+            if (!wide) {   // the rows of the gradient lie otherwise in memory than those of the logits (unsigned: a step past the largest vocabulary fits)
+                for (unsigned j = from + tid; j < (unsigned)to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
                 return;
             }
             const bool resident = STATS && groups <= 4;
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                     for (int i = v_first; i < sl.v1; i += TEAM) store_pack<T, VEC>(grad + sl.head + (long long)i * VEC, o);
                     if (r_at >= 0) grad[r_at] = o.v[0];
                 } else {
-                    for (int j = from + tid; j < to; j += TEAM) grad[j] = o.v[0];
+                    for (unsigned j = from + tid; j < (unsigned)to; j += TEAM) grad[j] = o.v[0];
                 }
             }
         } else {

@@ -149,3 +149,22 @@ def test_backward_walks_over_many_small_rows(cuda_device, dtype):
     logits, indices, teacher = make(20000, 10, 4, dtype, 6, cuda_device)
     check(logits, indices, teacher, 2.0, reduction="batchmean", up=torch.tensor(2.5, device=cuda_device))
     check(logits, indices, teacher, 2.0, reduction="batchmean")
+
+
+def test_the_largest_vocabulary(cuda_device):
+    """2^31 - 1 equal logits that start off a 16-byte boundary: the step past the last one stays in range."""
+    from geo_b200 import functional as F
+
+    vocab = 2 ** 31 - 1
+    logits = torch.zeros(vocab + 1, dtype=torch.bfloat16, device=cuda_device)[1:].view(1, vocab).requires_grad_(True)
+    indices = torch.tensor([[5, vocab - 1, 2 ** 30]], device=cuda_device)
+    teacher = torch.zeros(1, 3, device=cuda_device)
+    loss = F.distillation_loss(logits, indices, teacher, reduction="none")
+    assert abs(float(loss.detach()) - (31 * math.log(2) - math.log(3))) <= 22 * 2.0 ** -15
+    (grad,) = torch.autograd.grad(loss, logits, torch.ones(1, device=cuda_device))
+    assert (grad[0, indices[0]].double() + 1 / 3).abs().max() <= 2.0 ** -8
+    assert int((grad == 2.0 ** -31).sum()) == vocab - 3      # 1 / vocab in 16 bits
+    del grad
+    loss = F.distillation_loss(logits, indices, teacher, weight=torch.zeros(1, device=cuda_device), reduction="none")
+    (grad,) = torch.autograd.grad(loss, logits, torch.ones(1, device=cuda_device))
+    assert float(loss.detach()) == 0 and int(torch.count_nonzero(grad)) == 0
