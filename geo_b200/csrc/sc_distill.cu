@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         }
 
         float m = 0.f, sum = 0.f;
-        bool flat = false;   // m c out of range: a logit is either m or nothing, or NaN
-        auto seen = [&](float v) { return !flat ? v : v < m ? NEG_INF : v - m; };   // a NaN stays one
+        bool flat = false;   // m c out of range: a logit is either m or nothing (one that is NaN makes the sum NaN)
+        auto seen = [&](float v) { return !flat ? v : v == m ? 0.f : NEG_INF; };
         auto out_of_range = [&]() { return fabsf(m) <= 3.402823466e38f && !(fabsf(scaled(m)) <= FAR); };
         // Largest logit and sum of the warp.  A thread's reference is the first largest value that it meets, and moves only
         // for one that is 2^32 times as probable (some lane would move it at nearly every vector otherwise); sums stay far
@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             constexpr bool FLAT = decltype(is_flat)::value;
             float top = r_at >= 0 ? seen(r_value) : NEG_INF, ref = scaled(top), base = base_of(ref), s1 = 0.f;
             float s0 = r_at >= 0 ? ex2(fmaf(top, c, -base)) : 0.f;
+            if (FLAT && r_value != r_value) s1 = r_value;
             auto look = [&](float large) {
                 top = fmaxf(top, large);
                 if (scaled(large) > ref + 32.f) {
@@ -345,7 +346,10 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                 unpack<VEC>(load_staged<T, VEC>(at), f);
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    if (FLAT) f[e] = seen(f[e]);
+                    if (FLAT) {
+                        if (f[e] != f[e]) s1 = f[e];
+                        f[e] = seen(f[e]);
+                    }
                     large = fmaxf(large, f[e]);
                 }
                 look(large);
@@ -415,8 +419,8 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
         const float ref = flat ? 0.f : scaled(m), inv_s = 1.f / sum, a = GRAD ? up * pr.grad_factor * w * pr.temperature : 0.f, a_s = a * inv_s;
         const bool wide = GRAD && ((uintptr_t)(grad + sl.head) & 15) == 0;
         auto give_all = [&]() {   // the gradient apart from the teacher's share
-            if (!wide) {   // the rows of the gradient lie otherwise in memory than those of the logits (unsigned: a step past the largest vocabulary fits)
-                for (unsigned j = from + tid; j < (unsigned)to; j += TEAM) grad[j] = from_float<T>(ex2(fmaf(seen(to_float(z[j])), c, -ref)) * a_s);
+            if (!wide) {   // the rows of the gradient lie otherwise in memory than those of the logits (from the slice's start, so that no step leaves 31 bits)
+                for (int j = tid; j < to - from; j += TEAM) grad[from + j] = from_float<T>(ex2(fmaf(seen(to_float(z[from + j])), c, -ref)) * a_s);
                 return;
             }
             const bool resident = STATS && groups <= 4;
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
                     for (int i = v_first; i < sl.v1; i += TEAM) store_pack<T, VEC>(grad + sl.head + (long long)i * VEC, o);
                     if (r_at >= 0) grad[r_at] = o.v[0];
                 } else {
-                    for (unsigned j = from + tid; j < (unsigned)to; j += TEAM) grad[j] = o.v[0];
+                    for (int j = tid; j < to - from; j += TEAM) grad[from + j] = o.v[0];
                 }
             }
         } else {
@@ -476,11 +480,12 @@ __global__ void __launch_bounds__(team_threads(TEAM), team_blocks(TEAM, GRAD)) d
             if (STATS && GRAD && scribe) merge_entries(en, pr.top, from, to, psum);
             if (STATS && scribe && rank == 0) {
                 const double log_s = logf(sum), log_p = logf(psum);   // half a step of about 10 at most: what is added to them is exact
-                const double largest = flat ? (double)m * (double)c : (double)ref;   // what S is taken against
+                // a logit's share of log q against what S is taken against, halved: the difference stays in range
+                auto half_apart = [&](float v) { return (double)(flat ? 0.5f * v - 0.5f * m : 0.5f * v); };
                 double loss = 0;
                 for (int k = lane; k < pr.top; k += 32)
                     if (en.idx[k] >= 0 && en.prob[k] > 0.f)
-                        loss += (double)(en.prob[k] / psum) * (((double)en.diff[k] - log_p) - (((double)en.own[k] * (double)c - largest) * 0.6931471805599453 - log_s));
+                        loss += (double)(en.prob[k] / psum) * (((double)en.diff[k] - log_p) - ((half_apart(en.own[k]) * (double)(2 * c) - (double)ref) * 0.6931471805599453 - log_s));
                 loss = warp_sum(loss);
                 if (lane == 0) {
                     const double t = pr.temperature;

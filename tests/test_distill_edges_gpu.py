@@ -51,6 +51,9 @@ def test_far_rows_by_hand(cuda_device):
     assert abs(float(loss) - 1e-12 * (5e5 - math.log(2))) <= 5e-7 * 2.0 ** -20
     loss = F.distillation_loss(torch.tensor([[2e9, 1e9, 0.0, 1.0]], device=cuda_device), entries, equal)
     assert abs(float(loss) - 5e8) <= 5e8 * 2.0 ** -20
+    # the two ends of the type, further apart than the type reaches: T (6e38 / 2)
+    loss = F.distillation_loss(torch.tensor([[3e38, -3e38, 0.0, 1.0]], device=cuda_device), entries, equal, 1e-3)
+    assert abs(float(loss) - 3e35) <= 3e35 * 2.0 ** -20
     # a student that rules the second entry out
     loss = F.distillation_loss(torch.tensor([[2e9, -math.inf, 0.0, 1.0]], device=cuda_device), entries, equal)
     assert float(loss) == math.inf
