@@ -20,7 +20,8 @@
 //
 // Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
 // out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the
-// CTA stops waiting, lets its own copies and instructions in flight finish (again with a bound) and leaves.
+// CTA (or pair) stops waiting.  When all its warps have stopped, whichever of them it was that gave up, the copies that were
+// asked for and the instructions that were issued get their time to finish (again with a bound) before a CTA leaves.
 #include <cuda.h>
 
 #include <algorithm>
@@ -85,9 +86,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
     return false;
 }
-// After an abort: whatever is still in flight towards `bar` gets its time to arrive.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < LT_SPIN_LIMIT && !mbar_try_wait(bar, parity); i++) {}
+// After an abort: whatever is still in flight towards `bar` gets its time to arrive, out of `left` looks for all of them.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, int &left) {
+    while (left > 0 && !mbar_try_wait(bar, parity)) left--;
 }
 
 template <int CTAS> __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
@@ -172,6 +173,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __shared__ __align__(16) float split_x[SPLIT ? BN : 1], split_w[SPLIT ? 128 : 1], split_b[SPLIT ? 128 : 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ __align__(16) int other[4];   // of the pair's other CTA, told at the end: whether it gave up, stages it asked for
     const uint32_t tiles = (smem_u32(lt_smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);
@@ -219,17 +221,17 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const uint32_t tmem_base = CTAS == 1 && warp == 0 ? 0 : tmem_slot;   // not that warp's to read
     const int all_kb = (pr.k + LT_KB - 1) / LT_KB;
     after_previous();
+    int asked = 0;   // stages that this CTA has asked for (in the thread that asks)
     const int kb0 = SPLIT ? all_kb * part / splits : 0, kb1 = SPLIT ? all_kb * (part + 1) / splits : all_kb;   // all_kb <= 1024
 
     if (warp == 0) {
         if (lane == 0) {
-            int it = 0;
             bool ok = true;
             for (int t = worker; t < ntiles && ok; t += workers) {
                 const int n0 = (t % ntiles_n) * 128 * CTAS + rank * 128, m0 = (t / ntiles_n) * BN + rank * Tile::X_ROWS;
-                for (int kb = kb0; kb < kb1; kb++, it++) {
-                    const int s = it % ST;
-                    if (!(ok = mbar_wait(empty_bar(s), ((it / ST) & 1) ^ 1, abort))) break;
+                for (int kb = kb0; kb < kb1; kb++, asked++) {
+                    const int s = asked % ST;
+                    if (!(ok = mbar_wait(empty_bar(s), ((asked / ST) & 1) ^ 1, abort))) break;
                     if (rank == 0) mbar_expect_tx(full_bar(s), (uint32_t)(CTAS * Tile::STAGE));
                     const uint32_t dst = tiles + (uint32_t)s * Tile::STAGE;
                     const uint32_t bar = CTAS == 1 ? full_bar(s) : rank0_address(full_bar(s));
@@ -237,8 +239,6 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     tma_load<CTAS>(dst + 128 * LT_KB, &map_x, bar, kb * LT_KB, m0);
                 }
             }
-            if (!ok && rank == 0)   // the stages that were asked for last
-                for (int i = it < ST ? 0 : it - ST; i < it; i++) mbar_drain(full_bar(i % ST), (i / ST) & 1);
         }
         __syncwarp();
         cluster_begun();
@@ -261,10 +261,6 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                     umma_commit<CTAS>(empty_bar(s));
                 }
                 if (ok) umma_commit<CTAS>(accf_bar(a));
-            }
-            if (!ok) {   // instructions in flight read shared memory and write tensor memory
-                umma_commit<CTAS>(drain_bar);
-                mbar_drain(drain_bar, 0);
             }
         }
         __syncwarp();
@@ -370,7 +366,23 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
+    if (CTAS == 2 && threadIdx.x == 0) store_remote(smem_u32(other), rank ^ 1, abort_flag, asked, 0, 0);
     tile_sync<CTAS == 2 || SPLIT>();   // nobody leaves while another CTA may still reach its barriers; SPLIT: all parts are there
+    if (abort_flag || (CTAS == 2 && other[0])) {   // the same for both of a pair
+        int left = LT_SPIN_LIMIT;
+        if (rank == 0 && threadIdx.x == 0) {   // copies: the stages that were asked for last, by either
+            const int last = CTAS == 2 ? max(asked, other[1]) : asked;
+            for (int i = last < ST ? 0 : last - ST; i < last; i++) {
+                if (i >= asked) mbar_expect_tx(full_bar(i % ST), (uint32_t)Tile::STAGE);   // by the odd CTA alone
+                mbar_drain(full_bar(i % ST), (i / ST) & 1, left);
+            }
+        } else if (rank == 0 && threadIdx.x == 32) {   // instructions: they read shared memory and write tensor memory
+            umma_commit<CTAS>(drain_bar);
+            mbar_drain(drain_bar, 0, left);
+        }
+        __syncthreads();
+        tile_sync<CTAS == 2>();
+    }
     if (SPLIT) {
         // a warp adds up 32 channels of four tokens
         const int n0 = (worker % ntiles_n) * 128, m0 = (worker / ntiles_n) * BN + part * share;

@@ -84,3 +84,20 @@ def test_scale_of_a_sum_that_leaves_the_range_is_refused():
         F.distillation_loss(torch.zeros(4096, 8), *entries, reduction="sum", scale=1e36)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         F.distillation_loss(torch.zeros(4096, 8), *entries, reduction="batchmean", scale=1e36)
+
+
+def test_no_thread_block_leaves_with_copies_or_instructions_in_flight():
+    """What a wait that runs out leaves behind is waited for (with a bound) after the roles of all warps, whichever of them
+    gave up, and before tensor memory is freed."""
+    import os
+    import re
+
+    with open(os.path.join(os.path.dirname(os.path.abspath(layers.__file__)), "csrc", "sc_linear_int8_tc.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    kernel = code[code.index("linear_int8_tc_kernel(") : code.index("EncodeTiledFn encode_fn")]
+    roles, end = kernel[: kernel.rindex("mbar_arrive_leader")], kernel[kernel.rindex("mbar_arrive_leader") :]
+    assert "mbar_drain" not in roles
+    order = [end.index(step) for step in ("__syncthreads();", "store_remote(smem_u32(other)", "tile_sync<CTAS == 2 || SPLIT>();", "if (abort_flag || ",
+                                          "mbar_drain(full_bar", "umma_commit<CTAS>(drain_bar)", "mbar_drain(drain_bar", "tile_sync<CTAS == 2>();",
+                                          "tmem_free<CTAS>")]
+    assert order == sorted(order)
