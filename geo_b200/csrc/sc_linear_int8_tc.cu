@@ -303,7 +303,7 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 __syncwarp();
                 ask_scales(t + workers);
             }
-            if (!mbar_wait(accf_bar(a), (n >> 1) & 1, abort)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(a), (n >> 1) & 1, abort))) break;   // a warp stops as a whole
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             T *out = (T *)pr.out + (long long)m0 * pr.out_stride + ch;
             const bool paired = sizeof(T) == 2 && pr.out_stride % 2 == 0 && pr.n % 2 == 0 && ((uintptr_t)pr.out & 3) == 0;

@@ -101,3 +101,13 @@ def test_no_thread_block_leaves_with_copies_or_instructions_in_flight():
                                           "mbar_drain(full_bar", "umma_commit<CTAS>(drain_bar)", "mbar_drain(drain_bar", "tile_sync<CTAS == 2>();",
                                           "tmem_free<CTAS>")]
     assert order == sorted(order)
+
+
+def test_a_warp_that_reads_tensor_memory_stops_as_a_whole():
+    """The reads are instructions of a whole warp: its lanes, which look at the barrier and the flag one by one, agree first."""
+    import os
+    import re
+
+    with open(os.path.join(os.path.dirname(os.path.abspath(layers.__file__)), "csrc", "sc_linear_int8_tc.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert re.findall(r"if \(!(.*?)mbar_wait\(accf_bar", code) == ["__all_sync(0xffffffffu, "]
