@@ -583,6 +583,7 @@ int geo_sc_distill_forward(long long rows, int vocab, int top, int dtype, const 
     int rc = check_distill(rows, vocab, top, dtype, logits, stride, indices, index_bits, teacher, teacher_dtype, temperature);
     if (rc) return rc;
     if ((rows > 0 && (!row_loss || !stats)) || (mean && !loss)) return fail(GEO_SC_ERR_NULL, "row_loss, stats and the loss are required");
+    if (!aligned_to(stats, 8)) return fail(GEO_SC_ERR_UNSUPPORTED, "stats has to start on an 8-byte boundary");
     cudaStream_t s = (cudaStream_t)stream;
     const double all = mean ? (double)scale / (double)(rows > 0 ? rows : 1) : (double)scale;
     if (rows > 0) {
@@ -607,6 +608,7 @@ int geo_sc_distill_backward(long long rows, int vocab, int top, int dtype, const
     if (rc) return rc;
     if (rows == 0) return GEO_SC_OK;
     if (!stats || !upstream || !grad) return fail(GEO_SC_ERR_NULL, "stats, upstream and grad are required");
+    if (!aligned_to(stats, 8)) return fail(GEO_SC_ERR_UNSUPPORTED, "stats has to start on an 8-byte boundary");
     DistillParams p = {};
     p.logits = logits; p.indices = indices; p.teacher = teacher; p.weight = weight; p.upstream = upstream;
     p.stats = (float2 *)const_cast<void *>(stats); p.grad = grad;

@@ -391,7 +391,8 @@ int geo_sc_linear_int8(int m, int n, int k, const int8_t *x_device, long long x_
  * 0; an index >= vocab or a teacher's logit that is NaN or +inf gives the row a loss and a gradient of NaN.
  * mean != 0: loss[0] = scale * (sum of the row losses) / rows (0 rows: 0), added in a fixed order; row_loss [rows]
  * receives the unscaled row losses.  mean == 0: row_loss receives scale * row loss.  stats: 8 bytes per row for the
- * backward pass.  grad ([rows][vocab] dense, or NULL): the gradient for an upstream gradient of 1. */
+ * backward pass, on an 8-byte boundary (GEO_SC_ERR_UNSUPPORTED otherwise).  grad ([rows][vocab] dense, or NULL): the
+ * gradient for an upstream gradient of 1. */
 int geo_sc_distill_forward(long long rows, int vocab, int top, int dtype, const void *logits_device, long long stride,
                            const void *indices_device, int index_bits, const void *teacher_device, int teacher_dtype,
                            const float *weight_device, float temperature, float scale, int mean, float *row_loss_device,

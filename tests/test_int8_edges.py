@@ -111,3 +111,14 @@ def test_a_warp_that_reads_tensor_memory_stops_as_a_whole():
     with open(os.path.join(os.path.dirname(os.path.abspath(layers.__file__)), "csrc", "sc_linear_int8_tc.cu")) as f:
         code = re.sub(r"//[^\n]*", "", f.read())
     assert re.findall(r"if \(!(.*?)mbar_wait\(accf_bar", code) == ["__all_sync(0xffffffffu, "]
+
+
+def test_c_entry_points_refuse_stats_between_boundaries():
+    """The rows' statistics are read and written 8 bytes at a time (the pointers are never followed)."""
+    import ctypes
+
+    from geo_b200 import _lib
+
+    L, p, between, UNSUPPORTED = _lib.lib(), ctypes.c_void_p(4096), ctypes.c_void_p(4100), -9
+    assert L.geo_sc_distill_forward(1, 8, 3, 0, p, 8, p, 64, p, 0, None, 1.0, 1.0, 1, p, between, p, None, None) == UNSUPPORTED
+    assert L.geo_sc_distill_backward(1, 8, 3, 0, p, 8, p, 64, p, 0, None, 1.0, 1.0, 1, between, p, 0, p, None) == UNSUPPORTED
