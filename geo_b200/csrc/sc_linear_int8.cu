@@ -11,8 +11,10 @@
 // into fragments.  The order of k inside a product is free, so a lane takes 16 consecutive bytes of its weight row and
 // the same 16 bytes of its token rows for two instructions: whole 16-byte loads, no shared memory, no shuffles.  A CTA
 // of eight warps owns 16 channels and all tokens; the warps split k and join their integer sums in shared memory.
-// Bound by the weights' bytes: 1 x 8192 x 8192 15.4 us (4.4 TB/s with the launch), 16 x 4096 x 4096 4.7 us.  Above 32
-// tokens the other kernel takes less (64 x 4096 x 4096: 7.9 us; 32 tokens: 6.6 here, 6.9 there).
+// Bound by the weights' bytes: 1 x 8192 x 8192 13.3 us (5.0 TB/s with the launch); with more tokens by the tokens' bytes
+// that every CTA reads again as well.  Measured by graph replay, here and on the other kernel: 32 x 1024 x 1024 2.7 and
+// 3.8 us, 9 x 4096 x 4096 5.9 and 5.9, 32 x 4096 x 4096 7.8 and 6.0, 16 x 8192 x 8192 16.0 and 14.5, 32 x 8192 x 8192 28.1
+// and 14.5.  The switch at 32 tokens is right for layers of about 1000 features and too high for wide ones.
 #include "sc_linear_int8.h"
 
 namespace geo {

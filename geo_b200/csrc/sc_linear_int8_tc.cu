@@ -13,10 +13,12 @@
 // (integers: the order of the additions does not matter).  Sending costs the sender no waiting; fetching the parts behind
 // the barrier took 3500 clocks more and a second barrier (256 x 4096 x 4096: 18 us against 12).
 //
-// What bounds it: the bytes that an SM takes in, about 50 a clock (a pair's stage of 32 KB per CTA takes 650 clocks, its
-// matrix instructions 512), which is why a pair shares its tokens and why small tiles on many SMs win over large tiles on
-// few as long as one turn holds them (choose_tile).  Measured: 8192 x 8192 x 8192 361 us = 3045 TOP/s (415 us under the power limit), 1024 x 4096 x 4096
-// 16 us, 256 x 4096 x 4096 12 us, 333 x 1001 x 2047 7.9 us.
+// What bounds it: with several turns of the pair's tile the time of a stage, 650 clocks for the 32 KB per CTA against 512 of
+// its matrix instructions.  With a single turn the start, 3.4 to 5.6 us, and then the stages, each 0.28 to 0.32 us whether
+// it brings 20 KB (32 tokens), 24 KB (64) or 32 KB (128, the pair): something fixed per stage and not the bytes, which has
+// not been traced further.  So small tiles on many SMs win over large tiles on few as long as one turn holds them
+// (choose_tile).  Measured: 8192 x 8192 x 8192 350 us = 3140 TOP/s at best, 400 to 450 us under the power limit,
+// 1024 x 4096 x 4096 15.3 us, 256 x 4096 x 4096 10.9 us, 333 x 1001 x 2047 6.8 us.
 //
 // Persistent CTAs; warp 0 issues the copies, warp 1 the matrix instructions, warps 2 to 9 read finished accumulators
 // out while the next tile fills the other buffer.  Every wait is bounded: one that runs out raises a count, and the

@@ -18,7 +18,7 @@
 // not grow with the row.  A row whose sum leaves the range of 32 bits (values above 1e18, or so small that their squares
 // vanish) is read and summed again in 64.
 //
-// Measured: 16384 x 8192 fp16 with residual 169 us = 5.6 TB/s, read back 60 us = 6.7 TB/s (of 6.46 for a plain copy).
+// Measured: 16384 x 8192 fp16 with residual 165 us = 5.7 TB/s, read back 61 us = 6.6 TB/s (of 6.46 for a plain copy).
 //
 // norm_int8_kernel: rows that start on 16-byte boundaries and are whole numbers of 16-byte vectors.  A thread copies the
 // vectors that it computes itself, so the stages need no barrier; the products stay in registers from the statistics to

@@ -188,7 +188,8 @@ def quantize_int8(x):
 
 
 def dequantize_int8(q, scale, dtype=torch.float32):
-    """The values ``q * scale`` that the integers of :func:`quantize_int8` and :func:`rms_norm_int8` stand for."""
+    """The values ``q * scale`` (the fp32 product, rounded to ``dtype``) that the integers of :func:`quantize_int8` and
+    :func:`rms_norm_int8` stand for."""
     return _rows().dequantize_int8(q, scale, dtype)
 
 
@@ -215,5 +216,9 @@ def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=N
     divided by the number of rows), ``'sum'`` or ``'none'``.
 
     ``scale`` is part of the loss; a loss scale or the loss's share in a sum is best given here, because the gradient
-    is computed along with the loss for an upstream gradient of 1 and again where that turns out to be another."""
+    is computed along with the loss for an upstream gradient of 1 and again where that turns out to be another.
+
+    ``temperature`` lies in [1e-6, 1e6].  The two logarithms are of sums in 32 bits, so that the loss of a row is off by
+    up to about 1e-6 ``T^2``: little beside losses of ``T^2`` times a divergence, but as much as the loss itself where
+    a temperature of hundreds leaves next to no divergence.  The gradient has no such factor."""
     return _rows().distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)

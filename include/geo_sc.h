@@ -370,7 +370,7 @@ int geo_sc_rms_norm_int8(long long rows, int cols, int dtype, const void *x_devi
 int geo_sc_quantize_int8(long long rows, int cols, int dtype, const void *x_device, long long x_stride, int8_t *q_device,
                          long long q_stride, float *scale_device, void *stream);
 
-/* out[row][col] = q * scale[row], rounded once to dtype; out is [rows][cols] dense. */
+/* out[row][col] = q * scale[row], the fp32 product rounded to dtype; out is [rows][cols] dense. */
 int geo_sc_dequantize_int8(long long rows, int cols, const int8_t *q_device, long long q_stride, const float *scale_device,
                            int dtype, void *out_device, void *stream);
 
