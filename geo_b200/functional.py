@@ -218,7 +218,7 @@ def distillation_loss(logits, indices, teacher_logits, temperature=1.0, weight=N
     ``scale`` is part of the loss; a loss scale or the loss's share in a sum is best given here, because the gradient
     is computed along with the loss for an upstream gradient of 1 and again where that turns out to be another.
 
-    ``temperature`` lies in [1e-6, 1e6].  The two logarithms are of sums in 32 bits, so that the loss of a row is off by
+    ``scale``, for ``'sum'`` times the number of rows, has to be finite in 32 bits; ``temperature`` lies in [1e-6, 1e6].  The two logarithms are of sums in 32 bits, so that the loss of a row is off by
     up to about 1e-6 ``T^2``: little beside losses of ``T^2`` times a divergence, but as much as the loss itself where
     a temperature of hundreds leaves next to no divergence.  The gradient has no such factor."""
     return _rows().distillation_loss(logits, indices, teacher_logits, temperature, weight, reduction, scale)
